@@ -38,6 +38,36 @@ class SampleParams(C.Structure):
         return cls(temperature, top_p, top_k, min_p, rep, freq, pres, softcap, precedence)
 
 
+class LossRows(C.Structure):
+    """struct geist_hip_loss_rows."""
+    _fields_ = [("d_logits", C.c_void_p), ("ld", C.c_size_t), ("rows", C.c_size_t),
+                ("n_vocab", C.c_size_t), ("type", C.c_int), ("d_allowed", C.c_void_p),
+                ("allowed_ld", C.c_size_t), ("temperature", C.c_float),
+                ("logit_softcap", C.c_float), ("d_grad", C.c_void_p), ("grad_ld", C.c_size_t)]
+
+
+class Teacher(C.Structure):
+    """struct geist_hip_teacher."""
+    _fields_ = [("d_ids", C.c_void_p), ("d_values", C.c_void_p), ("ld", C.c_size_t),
+                ("k", C.c_size_t), ("d_count", C.c_void_p), ("d_weight", C.c_void_p),
+                ("tail", C.c_int)]
+
+
+class Policy(C.Structure):
+    """struct geist_hip_policy."""
+    _fields_ = [("d_tokens", C.c_void_p), ("d_advantage", C.c_void_p), ("d_old", C.c_void_p),
+                ("d_ref", C.c_void_p), ("d_weight", C.c_void_p), ("clip_low", C.c_float),
+                ("clip_high", C.c_float), ("kl_coef", C.c_float), ("entropy_coef", C.c_float)]
+
+
+class Preference(C.Structure):
+    """struct geist_hip_preference."""
+    _fields_ = [("d_tokens", C.c_void_p), ("d_ref", C.c_void_p), ("d_seq_start", C.c_void_p),
+                ("n_pairs", C.c_size_t), ("d_weight", C.c_void_p), ("kind", C.c_int),
+                ("beta", C.c_float), ("margin", C.c_float), ("label_smoothing", C.c_float),
+                ("length_normalised", C.c_int)]
+
+
 class SpecResult(C.Structure):
     """struct geist_hip_spec_result."""
     _fields_ = [("token", C.c_int32), ("answered", C.c_int32), ("n_finalists", C.c_int32),
@@ -160,6 +190,13 @@ def load_library():
     lib.geist_hip_spec_head_view.argtypes = [vp, C.POINTER(SpecHeadView)]
     lib.geist_hip_spec_head_try.argtypes = [vp, vp, vp, i32, vp]
     lib.geist_hip_spec_head_try_hidden.argtypes = [vp, vp, vp, vp, f32, vp, i32, vp]
+    lib.geist_hip_loss_workspace_bytes.argtypes = [sz, sz]
+    lib.geist_hip_loss_workspace_bytes.restype = sz
+    lib.geist_hip_distill_rows.argtypes = [vp, C.POINTER(LossRows), C.POINTER(Teacher), vp, vp, sz]
+    lib.geist_hip_policy_loss_rows.argtypes = [vp, C.POINTER(LossRows), C.POINTER(Policy), vp, vp,
+                                               vp, vp, sz]
+    lib.geist_hip_preference_loss.argtypes = [vp, C.POINTER(LossRows), C.POINTER(Preference), vp,
+                                              vp, vp, vp, sz]
     _LIB = lib
     return lib
 
@@ -638,3 +675,115 @@ class HipSampler:
         self._check(self.lib.geist_hip_sampler_row_paths(self.h, out.ctypes.data_as(C.c_void_p),
                                                          int(rows)))
         return out
+
+    @staticmethod
+    def loss_workspace_bytes(rows, n_vocab):
+        """Bytes of scratch memory the losses need for rows x n_vocab logits."""
+        return int(load_library().geist_hip_loss_workspace_bytes(rows, n_vocab))
+
+    @staticmethod
+    def loss_rows(logits, grad=None, allowed=None, temperature=1.0, softcap=0.0):
+        """The rows of a loss: logits, and grad (or None: loss only) of the same shape and type, 2-D
+        float32, float16 or bfloat16 device tensors with consecutive row elements; grad may be
+        logits itself. allowed: as in rows()."""
+        assert logits.dim() == 2 and logits.stride(1) == 1 or logits.shape[1] == 1
+        r = LossRows()
+        r.type = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}[str(logits.dtype)]
+        r.d_logits = logits.data_ptr()
+        r.rows, r.n_vocab = logits.shape
+        r.ld = logits.stride(0) if r.rows > 1 else max(logits.stride(0), r.n_vocab)
+        r.temperature, r.logit_softcap = temperature, softcap
+        if allowed is not None:
+            assert allowed.dim() == 2 and allowed.stride(1) == 1 and allowed.element_size() == 4
+            assert allowed.shape[0] in (1, r.rows) and allowed.shape[1] * 32 >= r.n_vocab
+            r.d_allowed = allowed.data_ptr()
+            r.allowed_ld = 0 if allowed.shape[0] == 1 else allowed.stride(0)
+        if grad is not None:
+            assert grad.shape == logits.shape and grad.dtype == logits.dtype
+            assert grad.stride(1) == 1 or grad.shape[1] == 1
+            r.d_grad = grad.data_ptr()
+            r.grad_ld = grad.stride(0) if r.rows > 1 else max(grad.stride(0), r.n_vocab)
+        return r
+
+    @staticmethod
+    def _vector(t, n, dtype):
+        """Device address of a vector of n values, or None."""
+        if t is None:
+            return None
+        assert t.shape == (n,) and (t.stride(0) == 1 or n == 1) and str(t.dtype) == dtype, \
+            (tuple(t.shape), n, t.dtype)
+        return t.data_ptr()
+
+    @staticmethod
+    def teacher(ids, values, count=None, weight=None, tail=False):
+        """A teacher's lists: ids int32 and values float32, [rows, k]; count int32 [rows] entries of
+        them that count; weight float32 [rows]. tail: values are log-probabilities, and the mass that
+        is not listed counts as one more event."""
+        assert ids.shape == values.shape and ids.dim() == 2
+        assert str(ids.dtype) == "torch.int32" and str(values.dtype) == "torch.float32"
+        rows, k = ids.shape
+        assert (ids.stride(1) == 1 and values.stride(1) == 1) or k == 1
+        assert rows == 1 or ids.stride(0) == values.stride(0)
+        t = Teacher()
+        t.d_ids, t.d_values, t.k = ids.data_ptr(), values.data_ptr(), k
+        t.ld = max(ids.stride(0), k) if rows == 1 else ids.stride(0)
+        t.d_count = HipSampler._vector(count, rows, "torch.int32")
+        t.d_weight = HipSampler._vector(weight, rows, "torch.float32")
+        t.tail = int(tail)
+        return t
+
+    @staticmethod
+    def policy(tokens, advantage, old=None, ref=None, weight=None, clip_low=0.2, clip_high=0.2,
+               kl_coef=0.0, entropy_coef=0.0):
+        """Sampled tokens int32 [rows] (-1: not trained on) with their advantages; old and ref:
+        log-probabilities of the sampling and the reference policy (old None: the rows' own)."""
+        n = tokens.shape[0]
+        p = Policy()
+        p.d_tokens = HipSampler._vector(tokens, n, "torch.int32")
+        p.d_advantage = HipSampler._vector(advantage, n, "torch.float32")
+        p.d_old = HipSampler._vector(old, n, "torch.float32")
+        p.d_ref = HipSampler._vector(ref, n, "torch.float32")
+        p.d_weight = HipSampler._vector(weight, n, "torch.float32")
+        p.clip_low, p.clip_high = clip_low, clip_high
+        p.kl_coef, p.entropy_coef = kl_coef, entropy_coef
+        return p
+
+    @staticmethod
+    def preference(tokens, seq_start, ref=None, weight=None, kind="sigmoid", beta=0.1, margin=0.0,
+                   label_smoothing=0.0, length_normalised=False):
+        """Pairs of sequences: tokens int32 [rows] (-1: not counted), seq_start int32 [2 pairs + 1],
+        ref float32 [rows] log-probabilities of the reference model, weight float32 [pairs]. kind:
+        "sigmoid", "hinge" or "squared"."""
+        n_pairs = (seq_start.shape[0] - 1) // 2
+        p = Preference()
+        p.d_tokens = HipSampler._vector(tokens, tokens.shape[0], "torch.int32")
+        p.d_ref = HipSampler._vector(ref, tokens.shape[0], "torch.float32")
+        p.d_seq_start = HipSampler._vector(seq_start, 2 * n_pairs + 1, "torch.int32")
+        p.n_pairs = n_pairs
+        p.d_weight = HipSampler._vector(weight, n_pairs, "torch.float32")
+        p.kind = {"sigmoid": 0, "hinge": 1, "squared": 2}[kind]
+        p.beta, p.margin, p.label_smoothing = beta, margin, label_smoothing
+        p.length_normalised = int(length_normalised)
+        return p
+
+    @staticmethod
+    def _bytes(t):
+        return t.numel() * t.element_size() if t is not None else 0
+
+    def distill(self, rows, teacher, loss, workspace):
+        """loss: float32 [rows] or None; workspace: a device tensor of loss_workspace_bytes."""
+        self._check(self.lib.geist_hip_distill_rows(self.h, C.byref(rows), C.byref(teacher),
+                                                    _ptr(loss), _ptr(workspace),
+                                                    self._bytes(workspace)))
+
+    def policy_loss(self, rows, policy, loss, logprob, entropy, workspace):
+        """loss, logprob, entropy: float32 [rows] each, or None."""
+        self._check(self.lib.geist_hip_policy_loss_rows(
+            self.h, C.byref(rows), C.byref(policy), _ptr(loss), _ptr(logprob), _ptr(entropy),
+            _ptr(workspace), self._bytes(workspace)))
+
+    def preference_loss(self, rows, preference, loss, ratios, logprob, workspace):
+        """loss: float32 [pairs], ratios: float32 [2 pairs], logprob: float32 [rows], or None."""
+        self._check(self.lib.geist_hip_preference_loss(
+            self.h, C.byref(rows), C.byref(preference), _ptr(loss), _ptr(ratios), _ptr(logprob),
+            _ptr(workspace), self._bytes(workspace)))

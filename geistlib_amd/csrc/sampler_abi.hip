@@ -19,7 +19,9 @@
 #include <vector>
 
 #include "../../include/geist_lm_head_hip.h"
+#include "../../include/geist_loss_hip.h"
 #include "lm_head_kernels.h"
+#include "loss_kernels.h"
 #include "spec_head_kernels.h"
 #include "sampler_kernels.h"
 #include "sampler_host.h"
@@ -2542,6 +2544,61 @@ int geist_hip_sampler_row_paths(geist_hip_sampler *s, int32_t *h_paths, size_t r
     if (!s->cand.path)
         return fail(s, GEIST_HIP_E_INVALID_ARG, "no full-vocabulary top-p / min-p call was made yet");
     return geist_hip_download(s, h_paths, s->cand.path, rows * sizeof(int32_t));
+}
+
+/* ---- losses over logit rows ------------------------------------------------------------------ */
+size_t geist_hip_loss_workspace_bytes(size_t rows, size_t n_vocab) {
+    return loss_workspace_bytes(rows, n_vocab);
+}
+
+int geist_hip_distill_rows(geist_hip_sampler *s, const struct geist_hip_loss_rows *rows,
+                           const struct geist_hip_teacher *teacher, float *d_loss,
+                           void *d_workspace, size_t workspace_bytes) {
+    if (!s)
+        return GEIST_HIP_E_INVALID_ARG;
+    Refusal why;
+    int     rc = check_loss_rows(rows, d_workspace, workspace_bytes, d_loss, why);
+    if (rc == GEIST_HIP_OK)
+        rc = check_teacher(*rows, teacher, why);
+    if (rc != GEIST_HIP_OK)
+        return fail(s, rc, "distillation loss: %s", why.text);
+    HIPCHK(s, hipSetDevice(s->device));
+    launch_distill(*rows, *teacher, d_loss, d_workspace, s->stream);
+    return after_launch(s, "distillation loss");
+}
+
+int geist_hip_policy_loss_rows(geist_hip_sampler *s, const struct geist_hip_loss_rows *rows,
+                               const struct geist_hip_policy *policy, float *d_loss,
+                               float *d_logprob, float *d_entropy, void *d_workspace,
+                               size_t workspace_bytes) {
+    if (!s)
+        return GEIST_HIP_E_INVALID_ARG;
+    Refusal why;
+    int     rc = check_loss_rows(rows, d_workspace, workspace_bytes, d_loss, why);
+    if (rc == GEIST_HIP_OK)
+        rc = check_policy(policy, why);
+    if (rc != GEIST_HIP_OK)
+        return fail(s, rc, "policy loss: %s", why.text);
+    HIPCHK(s, hipSetDevice(s->device));
+    launch_policy(*rows, *policy, d_loss, d_logprob, d_entropy, d_workspace, s->stream);
+    return after_launch(s, "policy loss");
+}
+
+int geist_hip_preference_loss(geist_hip_sampler *s, const struct geist_hip_loss_rows *rows,
+                              const struct geist_hip_preference *preference, float *d_loss,
+                              float *d_ratios, float *d_logprob, void *d_workspace,
+                              size_t workspace_bytes) {
+    if (!s)
+        return GEIST_HIP_E_INVALID_ARG;
+    Refusal why;
+    int     rc = check_loss_rows(rows, d_workspace, workspace_bytes, d_loss, why);
+    if (rc == GEIST_HIP_OK)
+        rc = check_preference(preference, why);
+    if (rc != GEIST_HIP_OK)
+        return fail(s, rc, "preference loss: %s", why.text);
+    HIPCHK(s, hipSetDevice(s->device));
+    launch_preference(*rows, *preference, d_loss, d_ratios, d_logprob, d_workspace, s->stream);
+    return after_launch(s, "preference loss");
 }
 
 } /* extern "C" */
