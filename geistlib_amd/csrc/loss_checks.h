@@ -16,15 +16,16 @@
 
 namespace gs {
 
-/* What one workgroup found out about its part of a row. */
+/* What one workgroup found out about its part of a row. Values w = softcap(x) log2(e) / T. */
 struct LossPart {
-    double s;        /* sum of 2^((y - m) k); with a teacher's tail without the listed tokens */
-    double t;        /* sum of 2^u u, u = (y - m) k (entropy only) */
-    double a;        /* chunk 0: sum of q_j (y_j - m_listed) over the row's listed tokens; or y of the
-                      * sampled token */
-    double listed;   /* chunk 0, tail only: sum of 2^((y_j - m_listed) k) over the listed tokens */
-    float  m_listed; /* chunk 0: the largest listed y */
-    float  m;        /* the largest value summed, or one less than a fixed bound below it */
+    double s;       /* sum of 2^(w - c); with a teacher's tail without the listed tokens */
+    double t;       /* sum of 2^u u, u = w - c (entropy only) */
+    double c;       /* the reference, near the largest w */
+    double a;       /* chunk 0: sum of q_j (w_j - top) over the row's listed tokens; w of the sampled token */
+    double listed;  /* chunk 0, tail only: sum of 2^(w_j - top) over the listed tokens */
+    double top;     /* chunk 0: the largest listed w */
+    float  m;       /* careful: c = m log2(e) / T */
+    int    careful; /* the sums were made against a value m outside the range of plain references */
 };
 
 struct LossPlan {

@@ -1,0 +1,1133 @@
+/*
+ * loss_rows_kernels.h -- the kernels of the losses over logit rows (include/geist_loss_hip.h), as
+ * templates that loss_rows_f32.hip, loss_rows_f16.hip and loss_rows_bf16.hip instantiate.
+ *
+ * Every loss here needs of a row x the sum S = sum 2^(w_i - c) with w = softcap(x) k, k = log2(e) / T,
+ * against some reference c near the largest w (and, for the entropy, sum 2^u u with u = w - c), the
+ * values at a few listed tokens, and its gradient by the logits has one form:
+ *     g_i = (p_i (A + B u_i) - [i listed] q_i W) * softcap'(x_i) / T,     p_i = 2^u_i / S
+ * with A, B, W of the row (A differs between listed and other tokens for a teacher with a tail).
+ * So one streaming core serves all three: a pass that sums, a few scalars, a pass that writes.
+ *
+ *   k_loss_row   a workgroup per row does all of it; the row's first 16 groups of 16 bytes per thread
+ *                stay in registers between the passes, so that they are read once
+ *   k_loss_sums  the sums of a part of a row (few rows; preference loss)
+ *   k_loss_grad  the gradient of a part of a row from the parts' sums
+ */
+#ifndef GEIST_LOSS_ROWS_KERNELS_H
+#define GEIST_LOSS_ROWS_KERNELS_H
+
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+
+#include "loss_kernels.h"
+
+namespace gs {
+namespace {
+
+/* ---- types ---------------------------------------------------------------------------------- */
+typedef float    f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16   bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <int TYPE> struct Elem;
+template <> struct Elem<GEIST_HIP_TYPE_F32> {
+    typedef float         mem;
+    static constexpr int  N = 4;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f[i] = __uint_as_float(v[i]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = __float_as_uint(f[i]);
+        return v;
+    }
+    static __device__ __forceinline__ float one(mem x) { return x; }
+    static __device__ __forceinline__ mem   round(float x) { return x; }
+};
+template <> struct Elem<GEIST_HIP_TYPE_F16> {
+    typedef _Float16      mem;
+    static constexpr int  N = 8;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t) v[i]);
+            f[2 * i]      = (float) h[0];
+            f[2 * i + 1]  = (float) h[1];
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2 h = {(_Float16) f[2 * i], (_Float16) f[2 * i + 1]};
+            v[i]          = __builtin_bit_cast(uint32_t, h);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ float one(mem x) { return (float) x; }
+    static __device__ __forceinline__ mem   round(float x) { return (_Float16) x; }
+};
+template <> struct Elem<GEIST_HIP_TYPE_BF16> {
+    typedef __bf16        mem;
+    static constexpr int  N = 8;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i]     = __uint_as_float(v[i] << 16);
+            f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x2 p = {f[2 * i], f[2 * i + 1]};
+            v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+        }
+        return v;
+    }
+    static __device__ __forceinline__ float one(mem x) { return (float) x; }
+    static __device__ __forceinline__ mem   round(float x) { return (__bf16) x; }
+};
+
+/* ---- the workgroup -------------------------------------------------------------------------- */
+/* Orders LDS traffic only: the row's loads stay in flight across it, which __syncthreads() would wait
+ * for. */
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1)
+        v = fmax(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1)
+        v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1)
+        v += __shfl_xor(v, d);
+    return v;
+}
+constexpr int SLOTS = 16 * 4; /* doubles of LDS the reductions use: four per wavefront */
+/* over the workgroup; every thread gets the results */
+template <int THREADS, int K, bool MAX> __device__ __forceinline__ void block_reduce(double (&v)[K], double *slot) {
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+        v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
+    if constexpr (THREADS > 64) {
+        lds_barrier();
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                slot[(threadIdx.x >> 6) * 4 + i] = v[i];
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            v[i] = slot[(threadIdx.x & (THREADS / 64 - 1)) * 4 + i];
+#pragma unroll
+            for (int d = THREADS / 128; d; d >>= 1) {
+                const double o = __shfl_xor(v[i], d);
+                v[i]           = MAX ? fmax(v[i], o) : v[i] + o;
+            }
+        }
+    }
+}
+
+/* ---- a row ---------------------------------------------------------------------------------- */
+template <int TYPE> struct Row {
+    typedef typename Elem<TYPE>::mem mem;
+    static constexpr int             N = Elem<TYPE>::N;
+    const mem      *x;
+    mem            *g;
+    const uint32_t *allowed;
+    int             n, head, nvec; /* elements in front of the first 16-byte boundary, groups behind it */
+    bool            g_aligned;     /* the gradient's groups start on 16-byte boundaries too */
+    int             v0, v1;        /* this workgroup's groups */
+    bool            first, last;   /* it also takes the head / what is behind the last group */
+
+    __device__ Row(const LossArgs &a, int row, int chunk, int chunks, int chunk_vecs) {
+        x       = static_cast<const mem *>(a.x) + (long) row * a.ld;
+        g       = a.g ? static_cast<mem *>(a.g) + (long) row * a.gld : nullptr;
+        allowed = a.allowed ? a.allowed + (long) row * a.allowed_ld : nullptr;
+        n       = a.n;
+        head    = (int) ((16u - ((uintptr_t) x & 15u)) & 15u) / (int) sizeof(mem);
+        if (head > n)
+            head = n;
+        nvec      = (n - head) / N;
+        g_aligned = (((uintptr_t) (g + head)) & 15u) == 0;
+        v0        = min(nvec, chunk * chunk_vecs);
+        v1        = chunk == chunks - 1 ? nvec : min(nvec, v0 + chunk_vecs);
+        first     = chunk == 0;
+        last      = chunk == chunks - 1;
+    }
+    __device__ __forceinline__ int   elem0() const { return head + v0 * N; } /* of group v0 */
+    __device__ __forceinline__ u32x4 load(int v) const {
+        return *reinterpret_cast<const u32x4 *>(x + head + (long) v * N);
+    }
+    __device__ __forceinline__ void store(int v, u32x4 d) const {
+        mem *p = g + head + (long) v * N;
+        if (g_aligned) {
+            *reinterpret_cast<u32x4 *>(p) = d;
+        } else {
+            const mem *e = reinterpret_cast<const mem *>(&d);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                p[i] = e[i];
+        }
+    }
+    __device__ __forceinline__ bool may(int e) const {
+        return !allowed || ((allowed[e >> 5] >> (e & 31)) & 1u);
+    }
+    /* mask bits of the group that starts at element e */
+    __device__ __forceinline__ uint32_t bits(int e) const {
+        const int sh = e & 31;
+        uint32_t  w  = allowed[e >> 5] >> sh;
+        if (sh > 32 - N)
+            w |= allowed[(e >> 5) + 1] << (32 - sh);
+        return w;
+    }
+    /* the i-th element that belongs to no group: the head, then the tail; -1 behind them */
+    __device__ __forceinline__ int loose(int i) const {
+        if (first && i < head)
+            return i;
+        if (first)
+            i -= head;
+        const int behind = head + nvec * N;
+        return last && i < n - behind ? behind + i : -1;
+    }
+    /* whether element e is in the workgroup's part of the row */
+    __device__ __forceinline__ bool mine(int e) const {
+        const int lo = first ? 0 : elem0();
+        const int hi = last ? n : head + v1 * N;
+        return e >= lo && e < hi;
+    }
+};
+
+/* ---- values --------------------------------------------------------------------------------- */
+/* tanh(x / c) = 1 - 2 / (1 + E), E = 2^(2 x log2(e) / c): off by 1e-7 absolute, c 1e-7 in a capped
+ * logit, which a 16-bit gradient does not show. For f32 rows small arguments take the odd Taylor
+ * polynomial to z^13, relative error 2^-24 below 0.55. */
+__device__ __forceinline__ float cap_recip(const LossArgs &a, float x) { /* 1 / (1 + E) */
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.tanh_k));
+}
+__device__ __forceinline__ float accurate_tanh(const LossArgs &a, float x, float r) {
+    const float z = x * a.inv_cap, z2 = z * z;
+    float       p = 21844.0f / 6081075.0f;
+    p             = fmaf(p, z2, -1382.0f / 155925.0f);
+    p             = fmaf(p, z2, 62.0f / 2835.0f);
+    p             = fmaf(p, z2, -17.0f / 315.0f);
+    p             = fmaf(p, z2, 2.0f / 15.0f);
+    p             = fmaf(p, z2, -1.0f / 3.0f);
+    p             = fmaf(p * z2, z, z);
+    return fabsf(z) < 0.55f ? p : fmaf(-2.0f, r, 1.0f);
+}
+/* softcap(x) in binary32, as the degenerate rows' pass needs it */
+template <int FEAT> __device__ __forceinline__ float capped(const LossArgs &a, float x) {
+    return (FEAT & F_GENERAL) && a.cap > 0.0f ? a.cap * accurate_tanh(a, x, cap_recip(a, x)) : x;
+}
+/* softcap(x) k in binary64, for the few values a row's scalars are made of */
+template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const LossArgs &a, float x) {
+    if ((FEAT & F_GENERAL) && a.cap > 0.0f)
+        return (TYPE == GEIST_HIP_TYPE_F32 ? (double) a.cap * (double) a.k : (double) a.cap_k) *
+               tanh((double) x / (double) a.cap);
+    return (double) x * (double) a.k;
+}
+
+/* A group's exponents u = w - c, and 2^u; `keep` (general rows): bits of the tokens that count. r: what
+ * the soft-cap's slope is made of. */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_t keep, float c,
+                                           float (&e)[Elem<TYPE>::N], float (&u)[Elem<TYPE>::N],
+                                           float (&r)[Elem<TYPE>::N]) {
+    constexpr int N = Elem<TYPE>::N;
+    float         x[N];
+    Elem<TYPE>::unpack(raw, x);
+    if ((FEAT & F_GENERAL) && a.cap > 0.0f) {
+        const float at = a.cap_k - c;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r[i] = cap_recip(a, x[i]);
+            if (TYPE == GEIST_HIP_TYPE_F32)
+                u[i] = fmaf(a.cap * accurate_tanh(a, x[i], r[i]), a.k, -c);
+            else
+                u[i] = fmaf(-2.0f * a.cap_k, r[i], at);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            u[i] = fmaf(x[i], a.k, -c);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        e[i] = __builtin_amdgcn_exp2f(u[i]);
+    if ((FEAT & F_GENERAL) && a.bits) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t on = (uint32_t) ((int32_t) (keep << (31 - i)) >> 31);
+            e[i]              = __uint_as_float(__float_as_uint(e[i]) & on);
+            if (FEAT & F_ENTROPY)
+                u[i] = __uint_as_float(__float_as_uint(u[i]) & on);
+        }
+    }
+    if (FEAT & F_ENTROPY) { /* 0 * -inf is no term of an entropy */
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            u[i] = fmaxf(u[i], -1e30f);
+    }
+}
+/* Listed tokens of the workgroup's part of the row as bits (tail only): group v's start at bit
+ * (v - v0 + 1) N, so that a group's bits lie in one byte; the head is in front of group v0. */
+template <int N> __device__ __forceinline__ uint32_t listed_bits(const uint32_t *map, int group) {
+    const int at = (group + 1) * N;
+    return map[at >> 5] >> (at & 31);
+}
+template <int TYPE, int FEAT>
+__device__ __forceinline__ uint32_t keep_bits(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
+                                              int v) {
+    uint32_t keep = ~0u;
+    if ((FEAT & F_GENERAL) && a.bits) {
+        if (r.allowed)
+            keep = r.bits(r.head + v * Elem<TYPE>::N);
+        if (map)
+            keep &= ~listed_bits<Elem<TYPE>::N>(map, v - r.v0);
+    }
+    return keep;
+}
+
+/* ---- the pass that sums --------------------------------------------------------------------- */
+/* A thread sums 2^(w - c) against a reference c of its own, the largest w of its first group: later
+ * values that are larger only make larger terms, and a batch whose sum reaches 2^60 is done again
+ * behind a reference moved to its largest value. So the usual element costs a fused multiply-add, an
+ * exponential and an addition, and no maximum. A batch of U groups is added up in binary32 by halves,
+ * the batches in binary64: a running binary32 sum loses what is small beside a leading token, always
+ * downwards (2e-6 of the sum over a whole row, 1e-7 over batches of 32).
+ * References stay above -2^20 and should stay below 2^26, where c's rounding is harmless; rows for
+ * which that does not hold (nothing above -2^20, logits of 4e7 and more) are done again by
+ * careful_sums. */
+constexpr float C_LOW = -1048576.0f, C_HIGH = 67108864.0f, BATCH_HIGH = 0x1p60f;
+struct Acc {
+    float  c = C_LOW;
+    double s = 0.0, t = 0.0;
+};
+/* the largest value of a group that counts */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ float group_top(const LossArgs &a, u32x4 raw, uint32_t keep) {
+    float x[Elem<TYPE>::N], top = -INFINITY;
+    Elem<TYPE>::unpack(raw, x);
+#pragma unroll
+    for (int i = 0; i < Elem<TYPE>::N; ++i)
+        if (!(FEAT & F_GENERAL) || ((keep >> i) & 1u))
+            top = fmaxf(top, x[i]);
+    return capped<FEAT>(a, top); /* (it is monotone) */
+}
+__device__ __forceinline__ void acc_move(Acc &c, float top, float k) {
+    const float  w  = fmaxf(top * k, c.c);
+    const float  d  = c.c - w;
+    const double sc = (double) __builtin_amdgcn_exp2f(d);
+    c.t = sc * (c.t + (c.s == 0.0 ? 0.0 : c.s * (double) d));
+    c.s *= sc;
+    c.c = w;
+}
+/* COUNT groups, of which the j-th counts if live has bit j */
+template <int TYPE, int FEAT, int COUNT>
+__device__ __forceinline__ void acc_batch(const LossArgs &a, Acc &c, const u32x4 (&raw)[COUNT],
+                                          const uint32_t (&keep)[COUNT], uint32_t live) {
+    constexpr int N = Elem<TYPE>::N;
+    for (int tries = 0; tries < 2; ++tries) {
+        float s[COUNT], t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            s[j] = 0.0f;
+            if ((live >> j) & 1u) {
+                float e[N], u[N], r[N];
+                group_exps<TYPE, FEAT>(a, raw[j], keep[j], c.c, e, u, r);
+                if (FEAT & F_ENTROPY) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        t = fmaf(e[i], u[i], t);
+                }
+#pragma unroll
+                for (int half = N / 2; half; half >>= 1)
+#pragma unroll
+                    for (int i = 0; i < half; ++i)
+                        e[i] += e[i + half];
+                s[j] = e[0];
+            }
+        }
+#pragma unroll
+        for (int half = COUNT / 2; half; half >>= 1)
+#pragma unroll
+            for (int j = 0; j < half; ++j)
+                s[j] += s[j + half];
+        if (s[0] < BATCH_HIGH || tries == 1) {
+            c.s += (double) s[0];
+            if (FEAT & F_ENTROPY)
+                c.t += (double) t;
+            break;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j)
+            if ((live >> j) & 1u)
+                top = fmaxf(top, group_top<TYPE, FEAT>(a, raw[j], keep[j]));
+        acc_move(c, top, a.k);
+    }
+}
+template <int TYPE, int FEAT>
+__device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
+                                          Acc &c) {
+    if (threadIdx.x < 2 * Elem<TYPE>::N) {
+        const int e = r.loose((int) threadIdx.x);
+        const int at = e - r.elem0() + Elem<TYPE>::N;
+        if (e >= 0 && r.may(e) && !(map && ((map[at >> 5] >> (at & 31)) & 1u))) {
+            const float y = capped<FEAT>(a, Elem<TYPE>::one(r.x[e]));
+            if (y * a.k > c.c)
+                acc_move(c, y, a.k);
+            const float u = fmaf(y, a.k, -c.c), v = __builtin_amdgcn_exp2f(u);
+            c.s += (double) v;
+            if (FEAT & F_ENTROPY)
+                c.t += (double) v * (double) u;
+        }
+    }
+}
+/* the groups from v0 + `from` on, read as they come */
+template <int TYPE, int FEAT, int THREADS, int U>
+__device__ __forceinline__ void sum_groups(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
+                                           int from, Acc &c) {
+    bool start = from == 0;
+    for (int v = r.v0 + from + (int) threadIdx.x; v < r.v1; v += U * THREADS) {
+        u32x4    raw[U];
+        uint32_t keep[U], live = 0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            keep[j] = 0;
+            if (v + j * THREADS < r.v1) {
+                raw[j]  = r.load(v + j * THREADS);
+                keep[j] = keep_bits<TYPE, FEAT>(a, r, map, v + j * THREADS);
+                live |= 1u << j;
+            }
+        }
+        if (start)
+            acc_move(c, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
+        start = false;
+        acc_batch<TYPE, FEAT, U>(a, c, raw, keep, live);
+    }
+}
+
+/* A row's or a part's sums. Against c, or where `careful` against m k (which may be beyond binary32). */
+struct Sums {
+    double s, t;
+    float  c, m;
+    bool   careful;
+    double top;    /* the largest listed value, in exponents */
+    double listed; /* with a tail: the listed tokens' own sum against it */
+    __device__ __forceinline__ double ref(float k) const {
+        return careful ? (double) m * (double) k : (double) c;
+    }
+};
+/* The sums against c = ref + log2(s) instead, rounded: s is then near 1 and the exponents of the tokens
+ * that matter are small, so that they lose nothing to rounding when the gradient forms them again. */
+__device__ __forceinline__ void rebase(Sums &j) {
+    if (j.careful)
+        return;
+    const float  c  = (float) ((double) j.c + log2(j.s));
+    const double d  = (double) j.c - (double) c;
+    const double sc = exp2(d);
+    j.t = sc * (j.t + j.s * d);
+    j.s *= sc;
+    j.c = c;
+}
+/* Sums with the maximum known first and (y - m) k formed as a difference: any finite values. */
+template <int TYPE, int FEAT, int THREADS>
+__device__ __forceinline__ Sums careful_sums(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
+                                          double *slot) {
+    constexpr int N = Elem<TYPE>::N;
+    const int     lo = r.first ? 0 : r.elem0(), hi = r.last ? r.n : r.head + r.v1 * N;
+    auto counts = [&](int e) {
+        const int at = e - r.elem0() + N;
+        return r.may(e) && !(map && ((map[at >> 5] >> (at & 31)) & 1u));
+    };
+    double top[1] = {-FLT_MAX};
+    for (int e = lo + (int) threadIdx.x; e < hi; e += THREADS)
+        if (counts(e))
+            top[0] = fmax(top[0], (double) capped<FEAT>(a, Elem<TYPE>::one(r.x[e])));
+    block_reduce<THREADS, 1, true>(top, slot);
+    Sums j     = {};
+    j.careful  = true;
+    j.m        = (float) top[0];
+    double v[2] = {0.0, 0.0};
+    for (int e = lo + (int) threadIdx.x; e < hi; e += THREADS)
+        if (counts(e)) {
+            const float u = (capped<FEAT>(a, Elem<TYPE>::one(r.x[e])) - j.m) * a.k;
+            const float p = __builtin_amdgcn_exp2f(u);
+            v[0] += (double) p;
+            v[1] += (double) p * (double) fmaxf(u, -1e30f);
+        }
+    block_reduce<THREADS, 2, false>(v, slot);
+    j.s = v[0];
+    j.t = v[1];
+    return j;
+}
+/* the threads' sums, joined against the largest reference among them */
+template <int FEAT, int THREADS>
+__device__ __forceinline__ Sums join_threads(const Acc &c, double *slot) {
+    double top[1] = {(double) c.c};
+    block_reduce<THREADS, 1, true>(top, slot);
+    Sums j = {};
+    j.c    = (float) top[0];
+    const float  d  = c.c - j.c; /* (NaN beside +inf: so is the row) */
+    const double sc = (double) __builtin_amdgcn_exp2f(d);
+    if constexpr (FEAT & F_ENTROPY) {
+        double v[2] = {sc * c.s, sc * (c.t + (c.s == 0.0 ? 0.0 : c.s * (double) d))};
+        block_reduce<THREADS, 2, false>(v, slot);
+        j.s = v[0];
+        j.t = v[1];
+    } else {
+        double v[1] = {sc * c.s};
+        block_reduce<THREADS, 1, false>(v, slot);
+        j.s = v[0];
+    }
+    return j;
+}
+__device__ __forceinline__ bool needs_care(const Sums &j) { return !(j.c < C_HIGH) || j.s == 0.0; }
+/* the parts of a row, joined by every wavefront for itself */
+template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p, int chunks, float k) {
+    const int lane = threadIdx.x & 63;
+    double    top = -INFINITY;
+    float     m = -FLT_MAX;
+    bool      careful = false, plain = false;
+    for (int i = lane; i < chunks; i += 64) {
+        top = fmax(top, p[i].c);
+        careful |= p[i].careful != 0;
+    }
+    top = wave_max(top);
+    for (int i = lane; i < chunks; i += 64)
+        if (p[i].c == top) {
+            plain |= p[i].careful == 0;
+            if (p[i].careful)
+                m = fmaxf(m, p[i].m);
+        }
+    Sums j    = {};
+    j.careful = __any(careful);
+    plain     = __any(plain);
+    m         = wave_max(m);
+    /* (beside a plain part with the largest reference, any m near it will do) */
+    j.m = plain ? (float) (top / (double) k) : m;
+    j.c = (float) top;
+    const double ref = j.ref(k);
+    double s = 0.0, t = 0.0;
+    for (int i = lane; i < chunks; i += 64) {
+        const double d  = fmax(p[i].c - ref, -1e30);
+        const double sc = (double) __builtin_amdgcn_exp2f((float) d);
+        s += sc * p[i].s;
+        if (FEAT & F_ENTROPY)
+            t += sc * (p[i].t + p[i].s * d);
+    }
+    j.s      = wave_sum(s);
+    j.t      = (FEAT & F_ENTROPY) ? wave_sum(t) : 0.0;
+    j.top    = p[0].top;
+    j.listed = p[0].listed;
+    return j;
+}
+
+/* ---- the gradient --------------------------------------------------------------------------- */
+struct Coef {
+    float a;        /* 2^u_i (a + b u_i): 1 / S, 1 / T and the weight are in them */
+    float b;
+    float a_listed; /* 2^(w_j - top) a_listed - q_j q for listed tokens of a teacher */
+    float q;
+    bool  zero;     /* the row is written as zeros */
+};
+template <int TYPE, int FEAT>
+__device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32_t keep, const Coef &c,
+                                            float ref) {
+    constexpr int N = Elem<TYPE>::N;
+    float         e[N], u[N], r[N], g[N];
+    group_exps<TYPE, FEAT>(a, raw, keep, ref, e, u, r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        g[i] = e[i] * ((FEAT & F_ENTROPY) ? fmaf(c.b, u[i], c.a) : c.a);
+        if ((FEAT & F_GENERAL) && a.cap > 0.0f) /* 1 - tanh^2 = 4 (r - r^2) */
+            g[i] *= 4.0f * fmaf(-r[i], r[i], r[i]);
+        if ((FEAT & F_GENERAL) && a.bits) /* (a forbidden NaN has no slope either) */
+            g[i] = __uint_as_float(__float_as_uint(g[i]) &
+                                   (uint32_t) ((int32_t) (keep << (31 - i)) >> 31));
+    }
+    return Elem<TYPE>::pack(g);
+}
+template <int FEAT> __device__ __forceinline__ float cap_slope(const LossArgs &a, float x) {
+    if (!(FEAT & F_GENERAL) || !(a.cap > 0.0f))
+        return 1.0f;
+    const float r = cap_recip(a, x);
+    return 4.0f * fmaf(-r, r, r);
+}
+/* one element by any row's reference */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ float one_grad(const LossArgs &a, const Row<TYPE> &r, int e, float x,
+                                          const Coef &c, const Sums &j) {
+    if (!r.may(e))
+        return 0.0f;
+    const float y = capped<FEAT>(a, x);
+    const float u = j.careful ? (y - j.m) * a.k : fmaf(y, a.k, -j.c);
+    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, -1e30f), c.a) : c.a;
+    return __builtin_amdgcn_exp2f(u) * f * cap_slope<FEAT>(a, x);
+}
+/* the groups from v0 + `from` on, read again */
+template <int TYPE, int FEAT, int THREADS, int U>
+__device__ __forceinline__ void write_groups(const LossArgs &a, const Row<TYPE> &r, const Coef &c,
+                                             const Sums &j, int from) {
+    for (int v = r.v0 + from + (int) threadIdx.x; v < r.v1; v += U * THREADS) {
+        u32x4    raw[U];
+        uint32_t keep[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (v + i * THREADS < r.v1) {
+                raw[i]  = r.load(v + i * THREADS);
+                keep[i] = keep_bits<TYPE, FEAT>(a, r, nullptr, v + i * THREADS);
+            }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (v + i * THREADS < r.v1)
+                r.store(v + i * THREADS, group_grad<TYPE, FEAT>(a, raw[i], keep[i], c, j.c));
+    }
+}
+template <int TYPE, int FEAT>
+__device__ __forceinline__ void write_loose(const LossArgs &a, const Row<TYPE> &r, const Coef &c,
+                                            const Sums &j) {
+    if (threadIdx.x < 2 * Elem<TYPE>::N) {
+        const int e = r.loose((int) threadIdx.x);
+        if (e >= 0)
+            r.g[e] = Elem<TYPE>::round(one_grad<TYPE, FEAT>(a, r, e, Elem<TYPE>::one(r.x[e]), c, j));
+    }
+}
+/* rows of zeros, and rows whose sums careful_sums made */
+template <int TYPE, int FEAT, int THREADS>
+__device__ __forceinline__ void write_rare(const LossArgs &a, const Row<TYPE> &r, const Coef &c, const Sums &j) {
+    if (c.zero) {
+        for (int v = r.v0 + (int) threadIdx.x; v < r.v1; v += THREADS)
+            r.store(v, u32x4{0, 0, 0, 0});
+        const int e = threadIdx.x < 2 * Elem<TYPE>::N ? r.loose((int) threadIdx.x) : -1;
+        if (e >= 0)
+            r.g[e] = Elem<TYPE>::round(0.0f);
+        return;
+    }
+    const int lo = r.first ? 0 : r.elem0(), hi = r.last ? r.n : r.head + r.v1 * Elem<TYPE>::N;
+    for (int e = lo + (int) threadIdx.x; e < hi; e += THREADS)
+        r.g[e] = Elem<TYPE>::round(one_grad<TYPE, FEAT>(a, r, e, Elem<TYPE>::one(r.x[e]), c, j));
+}
+
+/* ---- one token per row ---------------------------------------------------------------------- */
+constexpr double LN2 = 0.693147180559945309417232;
+
+struct Token {
+    int    id; /* -1: none */
+    float  x;
+    double w; /* softcap(x) k; -inf where it is forbidden */
+};
+template <int TYPE, int FEAT>
+__device__ __forceinline__ Token load_token(const LossArgs &a, const Row<TYPE> &r, int row) {
+    Token t;
+    t.id = a.tokens[row];
+    t.x  = 0.0f;
+    t.w  = 0.0;
+    if (t.id < 0 || t.id >= r.n) {
+        t.id = -1;
+    } else if (!r.may(t.id)) {
+        t.w = -INFINITY;
+    } else {
+        t.x = Elem<TYPE>::one(r.x[t.id]);
+        t.w = value64<TYPE, FEAT>(a, t.x);
+    }
+    return t;
+}
+/* log p of the token; -inf where the row gives it nothing or has no distribution */
+__device__ __forceinline__ double token_logprob(double s, double ref, double w) {
+    return s == 0.0 ? -INFINITY : (w - ref - log2(s)) * LN2;
+}
+/* Policy loss of a row from its sums; `lead`: this thread writes the row's outputs. */
+__device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has_token, double tw,
+                                            const Sums &j, bool entropy, bool lead) {
+    const bool   empty = j.s == 0.0;
+    const double l2s   = empty ? 0.0 : log2(j.s);
+    const double lp    = !has_token ? 0.0 : empty ? -INFINITY : (tw - j.ref(a.k) - l2s) * LN2;
+    const double H     = entropy && !empty ? LN2 * (l2s - j.t / j.s) : 0.0;
+    const double w     = a.weight ? (double) a.weight[row] : 1.0;
+    Coef         c     = {0.0f, 0.0f, 0.0f, 0.0f, true};
+    double       loss  = 0.0;
+    if (w != 0.0 && has_token && lp != -INFINITY) {
+        const double A     = (double) a.advantage[row];
+        double       d     = 0.0;
+        const double ratio = a.old_lp ? exp(lp - (double) a.old_lp[row]) : 1.0;
+        if (A != 0.0) {
+            const double lo = 1.0 - (double) a.clip_low, hi = 1.0 + (double) a.clip_high;
+            const double held = ratio < lo ? lo : ratio > hi ? hi : ratio; /* NaN stays */
+            const double f = ratio * A, h = held * A;
+            loss = h < f ? -h : -f;
+            d    = h < f ? 0.0 : -f;
+        }
+        if (a.ref_lp) {
+            const double far = (double) a.ref_lp[row] - lp;
+            const double ex  = expm1(far);
+            loss += (double) a.kl_coef * (ex - far);
+            d -= (double) a.kl_coef * ex;
+        }
+        const double ec = (double) a.entropy_coef;
+        if (ec != 0.0)
+            loss -= ec * H;
+        loss *= w;
+        d *= w * a.inv_t;
+        const double be = w * ec * a.inv_t;
+        c.a = (float) ((be != 0.0 ? be * (H - l2s * LN2) - d : -d) / j.s);
+        c.b = (float) (be * LN2 / j.s);
+        c.q    = (float) -d;
+        c.zero = false;
+    }
+    if (lead) {
+        if (a.loss)
+            a.loss[row] = (float) loss;
+        if (a.logprob)
+            a.logprob[row] = (float) lp;
+        if (a.entropy)
+            a.entropy[row] = (float) H;
+    }
+    return c;
+}
+/* the token's own element, over what stands there */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ void write_token(const LossArgs &a, const Row<TYPE> &r, const Token &t,
+                                            const Coef &c, const Sums &j) {
+    const float u = (float) (t.w - j.ref(a.k));
+    const float g = __builtin_amdgcn_exp2f(u) * ((FEAT & F_ENTROPY) ? fmaf(c.b, u, c.a) : c.a) - c.q;
+    r.g[t.id] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, t.x));
+}
+
+/* ---- a teacher's list ----------------------------------------------------------------------- */
+/* In LDS, of each entry: its id (-1: left out), x, w - top (w = softcap(x) k, top the largest of them),
+ * its value, then q. `first`: a table of entries by id that keeps the first of a repeated id. */
+struct List {
+    int      *ids, *first;
+    float    *x, *u, *q;
+    uint32_t *map;
+    double    q_log_q, q_sum; /* sum q_j log q_j, sum q_j */
+    double    top;
+    double    q_u;            /* sum q_j (w_j - top) */
+    int       n;
+};
+/* row_top: the rows may hold their gradient already outside the workgroup's part; then only entries of
+ * that part are looked up, against this top. */
+template <int TYPE, int FEAT, int THREADS>
+__device__ __forceinline__ List load_list(const LossArgs &a, const Row<TYPE> &r, int row, void *lds,
+                                          double *slot, bool want_map,
+                                          const double *row_top = nullptr) {
+    List l;
+    l.ids   = static_cast<int *>(lds);
+    l.x     = reinterpret_cast<float *>(l.ids + a.list_k);
+    l.u     = l.x + a.list_k;
+    l.q     = l.u + a.list_k;
+    l.first = reinterpret_cast<int *>(l.q + a.list_k);
+    l.map   = reinterpret_cast<uint32_t *>(l.first + a.slots);
+    constexpr int N = Elem<TYPE>::N;
+    int           k = a.list_k;
+    if (a.count)
+        k = max(0, min(k, a.count[row]));
+    for (int i = threadIdx.x; i < a.slots; i += THREADS)
+        l.first[i] = -1;
+    const int span  = (r.last ? r.n : r.head + r.v1 * N) - r.elem0() + N; /* bits of the map */
+    const int words = want_map ? (span + 31) / 32 : 0;
+    for (int i = threadIdx.x; i < words; i += THREADS)
+        l.map[i] = 0u;
+    for (int j = threadIdx.x; j < k; j += THREADS) {
+        const int   id = a.ids[(long) row * a.list_ld + j];
+        const float v  = a.values[(long) row * a.list_ld + j];
+        const bool  ok = id >= 0 && id < r.n && v != -INFINITY && r.may(id);
+        l.ids[j]       = ok ? id : -1;
+        l.q[j]         = v;
+        l.x[j]         = ok && (!row_top || r.mine(id)) ? Elem<TYPE>::one(r.x[id]) : 0.0f;
+    }
+    lds_barrier();
+    for (int j = threadIdx.x; j < k; j += THREADS) {
+        const int id = l.ids[j];
+        if (id < 0)
+            continue;
+        uint32_t at = ((uint32_t) id * 2654435761u) & (uint32_t) (a.slots - 1);
+        for (;;) { /* ends: there are twice as many places as entries */
+            const int was = atomicCAS(&l.first[at], -1, j);
+            if (was == -1)
+                break;
+            if (l.ids[was] == id) { /* (whoever holds this place, now or later, lists this id) */
+                atomicMin(&l.first[at], j);
+                break;
+            }
+            at = (at + 1) & (uint32_t) (a.slots - 1);
+        }
+    }
+    lds_barrier();
+    double top[2] = {-INFINITY, -1e300};
+    bool   mine_out = false;
+    for (int j = threadIdx.x; j < k; j += THREADS) {
+        const int id = l.ids[j];
+        if (id < 0)
+            continue;
+        uint32_t at = ((uint32_t) id * 2654435761u) & (uint32_t) (a.slots - 1);
+        int      f;
+        while (l.ids[f = l.first[at]] != id)
+            at = (at + 1) & (uint32_t) (a.slots - 1);
+        if (f != j) {
+            mine_out = true; /* (the id stays until every thread has looked its own up) */
+            l.u[j]   = INFINITY;
+            continue;
+        }
+        const double w = value64<TYPE, FEAT>(a, l.x[j]);
+        top[0]         = fmax(top[0], (double) l.q[j]);
+        top[1]         = fmax(top[1], w);
+        l.u[j]         = 0.0f;
+        if (want_map && r.mine(id)) {
+            const int bit = id - r.elem0() + N;
+            atomicOr(&l.map[bit >> 5], 1u << (bit & 31));
+        }
+    }
+    block_reduce<THREADS, 2, true>(top, slot);
+    if (mine_out)
+        for (int j = threadIdx.x; j < k; j += THREADS)
+            if (l.u[j] == INFINITY)
+                l.ids[j] = -1;
+    l.top = row_top ? *row_top : top[1];
+    double v[3] = {0.0, 0.0, 0.0}; /* sums of e, e v, e u */
+    for (int j = threadIdx.x; j < k; j += THREADS)
+        if (l.ids[j] >= 0) {
+            const double z = a.tail ? (double) l.q[j] : ((double) l.q[j] - top[0]) * a.inv_t;
+            const double e = exp(z), u = value64<TYPE, FEAT>(a, l.x[j]) - l.top;
+            l.u[j]         = (float) u;
+            v[0] += e;
+            if (e != 0.0) {
+                v[1] += e * z;
+                v[2] += e * u;
+            }
+        }
+    block_reduce<THREADS, 3, false>(v, slot);
+    const double scale = a.tail || v[0] == 0.0 ? 1.0 : 1.0 / v[0];
+    for (int j = threadIdx.x; j < k; j += THREADS)
+        if (l.ids[j] >= 0) {
+            const double z = a.tail ? (double) l.q[j] : ((double) l.q[j] - top[0]) * a.inv_t;
+            l.q[j]         = (float) (exp(z) * scale);
+        }
+    l.q_sum   = v[0] * scale;
+    l.q_log_q = v[1] * scale - (a.tail || v[0] == 0.0 ? 0.0 : log(v[0]));
+    l.q_u     = v[2] * scale;
+    l.n       = k;
+    lds_barrier();
+    return l;
+}
+/* sum of 2^(w_j - top) of the listed tokens: apart from the others', so that neither mass is lost
+ * beside the other however far the two lie apart */
+template <int THREADS> __device__ __forceinline__ double listed_sum(const List &l, double *slot) {
+    double s[1] = {0.0};
+    for (int j = threadIdx.x; j < l.n; j += THREADS)
+        if (l.ids[j] >= 0)
+            s[0] += (double) __builtin_amdgcn_exp2f(l.u[j]);
+    block_reduce<THREADS, 1, false>(s, slot);
+    return s[0];
+}
+/* q_u and j.top (sum of q_j (w_j - top) and top) are handed in: the rows may have been replaced by
+ * their gradient since */
+__device__ __forceinline__ Coef distill_coef(const LossArgs &a, int row, const List &l, double q_u,
+                                             const Sums &j, bool lead) {
+    const double w   = a.weight ? (double) a.weight[row] : 1.0;
+    const double ref = j.ref(a.k);
+    /* everything against one reference: the listed tokens' sum and that of the rest */
+    const double base = a.tail && (j.s == 0.0 || j.top > ref) ? j.top : ref;
+    const double rest = j.s == 0.0 ? 0.0 : ref == base ? j.s : j.s * exp2(ref - base);
+    const double all  = a.tail ? rest + (j.top == base ? j.listed : j.listed * exp2(j.top - base)) : rest;
+    Coef   c    = {0.0f, 0.0f, 0.0f, 0.0f, true};
+    double loss = 0.0;
+    if (w != 0.0 && all != 0.0 && (a.tail || l.q_sum != 0.0)) {
+        const double l2s = log2(all);
+        /* sum q_j (log q_j - log p_j) */
+        loss = l.q_log_q + LN2 * (l.q_sum * (l2s + (base - j.top)) - q_u);
+        const double ws = w * a.inv_t;
+        c.a        = (float) (ws / all);
+        c.a_listed = (float) (ws / all * exp2(j.top - base));
+        if (a.tail) {
+            /* p_i (1 - q_rest / p_rest) = 2^(w_i - ref) / s * (p_rest - q_rest) */
+            const double q_rest = l.q_sum <= 1.0 ? 1.0 - l.q_sum : l.q_sum > 1.0 ? 0.0 : l.q_sum;
+            if (q_rest != 0.0)
+                loss += q_rest * (log(q_rest) -
+                                  (j.s == 0.0 ? -INFINITY : LN2 * (log2(j.s) + (ref - base) - l2s)));
+            c.a = j.s == 0.0 ? 0.0f : (float) (ws * (rest / all - q_rest) / j.s);
+        }
+        loss *= w;
+        c.q    = (float) ws;
+        c.zero = false;
+    }
+    if (lead && a.loss)
+        a.loss[row] = (float) loss;
+    return c;
+}
+template <int TYPE, int FEAT, int THREADS>
+__device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> &r, const List &l,
+                                             const Coef &c) {
+    for (int j = threadIdx.x; j < l.n; j += THREADS)
+        if (l.ids[j] >= 0 && r.mine(l.ids[j])) {
+            const float g = __builtin_amdgcn_exp2f(l.u[j]) * c.a_listed - l.q[j] * c.q;
+            r.g[l.ids[j]] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, l.x[j]));
+        }
+}
+
+/* ---- kernels -------------------------------------------------------------------------------- */
+/* A row per workgroup. The loads of what registers hold are all asked for at the start and are in
+ * flight while the teacher's list is read. */
+template <int OP, int FEAT> struct Held {
+    static constexpr int N = FEAT == (F_GENERAL | F_ENTROPY) ? 6
+                             : FEAT & F_GENERAL           ? 8
+                             : OP == OP_DISTILL           ? 12
+                                                          : 16;
+};
+constexpr int UH = 2;
+template <int TYPE, int OP, int FEAT, int THREADS>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_loss_row(LossArgs a) {
+    __shared__ double slot[SLOTS];
+    extern __shared__ __align__(16) char lds[];
+    constexpr int   HELD = Held<OP, FEAT>::N;
+    const int       row = blockIdx.x, tid = (int) threadIdx.x;
+    const Row<TYPE> r(a, row, 0, 1, 0);
+    u32x4           raw[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (h * THREADS + tid < r.nvec)
+            raw[h] = r.load(h * THREADS + tid);
+    List  l;
+    Token t;
+    if constexpr (OP == OP_DISTILL)
+        l = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, (FEAT & F_GENERAL) && a.tail);
+    else
+        t = load_token<TYPE, FEAT>(a, r, row);
+    const uint32_t *map = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail ? l.map : nullptr;
+    Acc acc;
+#pragma unroll
+    for (int h = 0; h < HELD; h += UH) {
+        uint32_t keep[UH], live = 0;
+        u32x4    some[UH];
+#pragma unroll
+        for (int i = 0; i < UH; ++i) {
+            const int v = (h + i) * THREADS + tid;
+            keep[i]     = 0;
+            some[i]     = raw[h + i];
+            if (v < r.nvec) {
+                keep[i] = keep_bits<TYPE, FEAT>(a, r, map, v);
+                live |= 1u << i;
+            }
+        }
+        if (h == 0 && live)
+            acc_move(acc, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
+        acc_batch<TYPE, FEAT, UH>(a, acc, some, keep, live);
+        __builtin_amdgcn_sched_barrier(0); /* (interleaved, the batches would not fit the registers) */
+    }
+    sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, HELD * THREADS, acc);
+    acc_loose<TYPE, FEAT>(a, r, map, acc);
+    Sums j = join_threads<FEAT, THREADS>(acc, slot);
+    auto coef = [&]() {
+        if constexpr (OP == OP_DISTILL) {
+            j.top = l.top;
+            if (map)
+                j.listed = listed_sum<THREADS>(l, slot);
+            return distill_coef(a, row, l, l.q_u, j, tid == 0);
+        } else {
+            return policy_coef(a, row, t.id >= 0, t.w, j, FEAT & F_ENTROPY, tid == 0);
+        }
+    };
+    auto special = [&](const Coef &c) {
+        __syncthreads();
+        if constexpr (OP == OP_DISTILL)
+            write_listed<TYPE, FEAT, THREADS>(a, r, l, c);
+        else if (tid == 0)
+            write_token<TYPE, FEAT>(a, r, t, c, j);
+    };
+    if (needs_care(j)) { /* (what registers hold of the row is dead here) */
+        j            = careful_sums<TYPE, FEAT, THREADS>(a, r, map, slot);
+        const Coef c = coef();
+        if (r.g) {
+            __syncthreads();
+            write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
+            if (!c.zero)
+                special(c);
+        }
+        return;
+    }
+    rebase(j);
+    const Coef c = coef();
+    if (!r.g)
+        return;
+    __syncthreads(); /* every value of the row has been read before any is written */
+    if (c.zero) {
+        write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
+    } else {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const int v = h * THREADS + tid;
+            /* (hides that this is what the sums were made of: the compiler would keep the unpacked
+             * values, twice the registers) */
+            asm volatile("" : "+v"(raw[h]));
+            if (v < r.nvec)
+                r.store(v, group_grad<TYPE, FEAT>(a, raw[h], keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        write_groups<TYPE, FEAT, THREADS, 4>(a, r, c, j, HELD * THREADS);
+        write_loose<TYPE, FEAT>(a, r, c, j);
+        special(c);
+    }
+}
+
+/* The sums of a part of a row. */
+template <int TYPE, int OP, int FEAT, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
+    __shared__ double slot[SLOTS];
+    extern __shared__ __align__(16) char lds[];
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    if constexpr (OP == OP_PREFERENCE) {
+        if (row < a.seq_start[0] || row >= a.seq_start[2 * a.n_pairs])
+            return;
+    }
+    const Row<TYPE> r(a, row, chunk, a.chunks, a.chunk_vecs);
+    const bool      tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    Acc             acc;
+    double          at = 0.0;
+    List            l = {};
+    if constexpr (OP == OP_DISTILL) {
+        if (tail || chunk == 0) {
+            l  = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, tail);
+            at = l.q_u;
+        }
+    } else if (chunk == 0) {
+        at = load_token<TYPE, FEAT>(a, r, row).w;
+    }
+    const uint32_t *map = tail ? l.map : nullptr;
+    sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, acc);
+    acc_loose<TYPE, FEAT>(a, r, map, acc);
+    Sums j = join_threads<FEAT, THREADS>(acc, slot);
+    if (needs_care(j))
+        j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, slot);
+    if (OP == OP_DISTILL && chunk == 0) {
+        j.top = l.top;
+        if (tail)
+            j.listed = listed_sum<THREADS>(l, slot);
+    }
+    if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.coef)
+        a.coef[row] = 0.0f;
+    if (threadIdx.x == 0)
+        a.part[(long) row * a.chunks + chunk] = {j.s, j.t, j.ref(a.k), at, j.listed, j.top, j.m, j.careful};
+}
+
+/* The gradient of a part of a row from the parts' sums; without one, a workgroup per row writes the
+ * row's outputs. */
+template <int TYPE, int OP, int FEAT, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, int chunk_vecs) {
+    __shared__ double slot[SLOTS];
+    extern __shared__ __align__(16) char lds[];
+    const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    if constexpr (OP == OP_PREFERENCE) {
+        if (row < a.seq_start[0] || row >= a.seq_start[2 * a.n_pairs])
+            return;
+    }
+    const LossPart *p  = a.part + (long) row * a.chunks;
+    Sums            j  = join_parts<FEAT>(p, a.chunks, a.k);
+    rebase(j);
+    const double    at = p[0].a;
+    const Row<TYPE> r(a, row, chunk, chunks, chunk_vecs);
+    const bool      lead = chunk == 0 && threadIdx.x == 0;
+    List            l    = {};
+    Token           t    = {-1, 0.0f, 0.0};
+    Coef            c;
+    if constexpr (OP == OP_DISTILL) {
+        l = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, false, &j.top);
+        c = distill_coef(a, row, l, at, j, lead);
+    } else {
+        const int  id        = a.tokens[row];
+        const bool has_token = id >= 0 && id < a.n;
+        if (has_token && r.g && r.mine(id))
+            t = load_token<TYPE, FEAT>(a, r, row);
+        if constexpr (OP == OP_PREFERENCE) {
+            const double d = (double) a.coef[row] * a.inv_t;
+            c              = {(float) (-d / j.s), 0.0f, 0.0f, (float) -d, d == 0.0};
+        } else {
+            c = policy_coef(a, row, has_token, at, j, FEAT & F_ENTROPY, lead);
+        }
+    }
+    if (!r.g)
+        return;
+    __syncthreads(); /* the part's values have been read before any is written */
+    if (c.zero || j.careful) {
+        write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
+    } else {
+        write_groups<TYPE, FEAT, THREADS, 4>(a, r, c, j, 0);
+        write_loose<TYPE, FEAT>(a, r, c, j);
+    }
+    if (c.zero)
+        return;
+    __syncthreads();
+    if constexpr (OP == OP_DISTILL) {
+        write_listed<TYPE, FEAT, THREADS>(a, r, l, c);
+    } else if (threadIdx.x == 0 && t.id >= 0) {
+        write_token<TYPE, FEAT>(a, r, t, c, j);
+    }
+}
+
+template <int TYPE, int OP, int FEAT>
+void launch_one(LossStage stage, const LossArgs &a, size_t lds, int chunks, int chunk_vecs, hipStream_t stream) {
+    if (stage == STAGE_ROW) {
+        if constexpr (OP != OP_PREFERENCE) {
+            const int need = a.n / Elem<TYPE>::N / Held<OP, FEAT>::N;
+            if (need <= 128)
+                k_loss_row<TYPE, OP, FEAT, 128><<<dim3(a.rows), 128, lds, stream>>>(a);
+            else if (need <= 256)
+                k_loss_row<TYPE, OP, FEAT, 256><<<dim3(a.rows), 256, lds, stream>>>(a);
+            else if (need <= 512)
+                k_loss_row<TYPE, OP, FEAT, 512><<<dim3(a.rows), 512, lds, stream>>>(a);
+            else
+                k_loss_row<TYPE, OP, FEAT, 1024><<<dim3(a.rows), 1024, lds, stream>>>(a);
+        }
+    } else if (stage == STAGE_SUMS) {
+        k_loss_sums<TYPE, OP, FEAT, 256><<<dim3((unsigned) a.rows * a.chunks), 256, lds, stream>>>(a);
+    } else {
+        k_loss_grad<TYPE, OP, FEAT, 256>
+            <<<dim3((unsigned) a.rows * chunks), 256, lds, stream>>>(a, chunks, chunk_vecs);
+    }
+}
+
+} // namespace
+
+template <int TYPE>
+void launch_loss(LossStage stage, int op, int feat, const LossArgs &a, size_t lds, int chunks,
+                 int chunk_vecs, hipStream_t stream) {
+#define GS_CASE(OP, FEAT)                                                                       \
+    if (op == OP && feat == (FEAT))                                                             \
+        return launch_one<TYPE, OP, (FEAT)>(stage, a, lds, chunks, chunk_vecs, stream);
+    GS_CASE(OP_TOKEN, 0)
+    GS_CASE(OP_TOKEN, F_ENTROPY)
+    GS_CASE(OP_TOKEN, F_GENERAL)
+    GS_CASE(OP_TOKEN, F_GENERAL | F_ENTROPY)
+    GS_CASE(OP_DISTILL, 0)
+    GS_CASE(OP_DISTILL, F_GENERAL)
+    GS_CASE(OP_PREFERENCE, 0)
+    GS_CASE(OP_PREFERENCE, F_GENERAL)
+#undef GS_CASE
+}
+
+} // namespace gs
+#endif /* GEIST_LOSS_ROWS_KERNELS_H */
