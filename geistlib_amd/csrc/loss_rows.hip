@@ -11,6 +11,7 @@
 #include <cstdint>
 
 #include "loss_kernels.h"
+#include "sampler_device.h"
 
 namespace gs {
 namespace {
@@ -18,62 +19,56 @@ namespace {
 constexpr double LN2   = 0.693147180559945309417232;
 constexpr double LOG2E = 1.44269504088896340735992;
 
-/* sum over the workgroup, every thread gets it; `slot`: a double per wavefront */
-template <int THREADS> __device__ __forceinline__ double block_sum(double v, double *slot) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1)
-        v += __shfl_xor(v, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        slot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = slot[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 64; ++i)
-        v += slot[i];
-    return v;
-}
-
 /* The pairs: log-probabilities of their rows, ratios, loss, and what each row's log-probability is
  * worth. */
-constexpr int PAIR_THREADS = 1024;
+constexpr int PAIR_THREADS = 512;
 __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
-    __shared__ double slot[16];
+    __shared__ double slot[4][PAIR_THREADS / 64];
     const int         pair = blockIdx.x;
-    double            ratio[2], share[2];
-    int               lo[2], hi[2];
     /* the rows that were summed: nothing outside them is looked at, whatever the starts between say */
     const int first = max(0, min(a.rows, a.seq_start[0]));
     const int last  = max(first, min(a.rows, a.seq_start[2 * a.n_pairs]));
-    for (int side = 0; side < 2; ++side) {
-        lo[side] = max(first, min(last, a.seq_start[2 * pair + side]));
-        hi[side] = max(lo[side], min(last, a.seq_start[2 * pair + side + 1]));
-        double sum = 0.0, n = 0.0;
-        for (int row = lo[side] + (int) threadIdx.x; row < hi[side]; row += PAIR_THREADS) {
-            const LossPart *p  = a.part + (long) row * a.chunks;
-            const int       id = a.tokens[row];
-            double          lp = 0.0;
-            if (id >= 0 && id < a.n) {
-                double c = p[0].c, s = 0.0;
-                for (int i = 1; i < a.chunks; ++i)
-                    c = fmax(c, p[i].c);
-                for (int i = 0; i < a.chunks; ++i)
-                    s += p[i].s * (double) __builtin_amdgcn_exp2f((float) fmax(p[i].c - c, -1e30));
-                lp = s == 0.0 ? -INFINITY : (p[0].a - c - log2(s)) * LN2;
-                if (lp != -INFINITY) {
-                    sum += a.ref_lp ? lp - (double) a.ref_lp[row] : lp;
-                    n += 1.0;
-                }
+    int       edge[3];
+    for (int i = 0; i < 3; ++i)
+        edge[i] = max(i ? edge[i - 1] : first, min(last, a.seq_start[2 * pair + i]));
+    double v[4] = {0.0, 0.0, 0.0, 0.0}; /* sums and numbers of tokens, of either side */
+    for (int row = edge[0] + (int) threadIdx.x; row < edge[2]; row += PAIR_THREADS) {
+        const LossPart *p    = a.part + (long) row * a.chunks;
+        const int       id   = a.tokens[row];
+        const bool      used = id >= 0 && id < a.n;
+        double          lp   = 0.0;
+        if (used) {
+            double c = p[0].c, s = 0.0;
+            for (int i = 1; i < a.chunks; ++i)
+                c = fmax(c, p[i].c);
+            for (int i = 0; i < a.chunks; ++i)
+                s += p[i].s * (double) __builtin_amdgcn_exp2f((float) fmax(p[i].c - c, -1e30));
+            lp = s == 0.0 ? -INFINITY : (p[0].a - c - log2(s)) * LN2;
+            if (lp != -INFINITY) {
+                const int side = row < edge[1] ? 0 : 1;
+                v[side] += a.ref_lp ? lp - (double) a.ref_lp[row] : lp;
+                v[2 + side] += 1.0;
             }
-            if (a.logprob)
-                a.logprob[row] = (float) lp;
-            if (a.coef) /* marks the rows that count */
-                a.coef[row] = (id >= 0 && id < a.n && lp != -INFINITY) ? 1.0f : 0.0f;
         }
-        sum         = block_sum<PAIR_THREADS>(sum, slot);
-        n           = block_sum<PAIR_THREADS>(n, slot);
-        share[side] = a.length_normalised ? 1.0 / fmax(n, 1.0) : 1.0;
-        ratio[side] = sum * share[side];
+        if (a.logprob)
+            a.logprob[row] = (float) lp;
+        if (a.coef) /* marks the rows that count */
+            a.coef[row] = used && lp != -INFINITY ? 1.0f : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = wave_sum_f64(v[i]);
+    if ((threadIdx.x & 63) == 0)
+        for (int i = 0; i < 4; ++i)
+            slot[i][threadIdx.x >> 6] = v[i];
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = wave_sum_f64((threadIdx.x & 63) < PAIR_THREADS / 64 ? slot[i][threadIdx.x & 63] : 0.0);
+    double ratio[2], share[2];
+    for (int side = 0; side < 2; ++side) {
+        share[side] = a.length_normalised ? 1.0 / fmax(v[2 + side], 1.0) : 1.0;
+        ratio[side] = v[side] * share[side];
     }
     const double gap = ratio[0] - ratio[1], beta = (double) a.beta;
     const double w = a.weight ? (double) a.weight[pair] : 1.0;
@@ -107,18 +102,22 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
             a.ratios[2 * pair + 1] = (float) ratio[1];
         }
     }
-    if (a.coef)
-        for (int side = 0; side < 2; ++side) {
-            const float c = (float) ((side ? -d : d) * w * share[side]);
-            for (int row = lo[side] + (int) threadIdx.x; row < hi[side]; row += PAIR_THREADS)
-                a.coef[row] = a.coef[row] != 0.0f ? c : 0.0f;
-        }
+    if (a.coef) {
+        const float c0 = (float) (d * w * share[0]), c1 = (float) (-d * w * share[1]);
+        for (int row = edge[0] + (int) threadIdx.x; row < edge[2]; row += PAIR_THREADS)
+            a.coef[row] = a.coef[row] == 0.0f ? 0.0f : row < edge[1] ? c0 : c1;
+    }
 }
 
 /* ---- launches ------------------------------------------------------------------------------- */
+/* The Infinity Cache holds 256 MB. Rows that cannot have come from it are read with non-temporal loads
+ * (729 MB of sums 138 -> 121 us); where a second pass follows, all but the last of them, which that pass
+ * reads first. */
+constexpr size_t CACHE_BYTES = (size_t) 224 << 20, KEPT_BYTES = (size_t) 160 << 20;
+
 size_t elem_bytes(int type) { return type == GEIST_HIP_TYPE_F32 ? 4 : 2; }
 
-LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
+LossArgs args_of(const geist_hip_loss_rows &r, void *ws, int cu_count) {
     LossArgs       a    = {};
     const LossPlan plan = loss_plan(r.rows, r.n_vocab, elem_bytes(r.type));
     a.x          = r.d_logits;
@@ -141,6 +140,10 @@ LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
     a.chunks     = plan.chunks;
     a.chunk_vecs = plan.chunk_vecs;
     a.part       = static_cast<LossPart *>(ws);
+    a.cu_count   = cu_count;
+    const size_t row_bytes = r.ld * elem_bytes(r.type);
+    a.streamed      = r.rows * row_bytes > CACHE_BYTES;
+    a.streamed_rows = a.streamed ? (int) (r.d_grad ? r.rows - KEPT_BYTES / row_bytes : r.rows) : 0;
     return a;
 }
 void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArgs &a, size_t lds,
@@ -159,8 +162,8 @@ void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArg
 } // namespace
 
 void launch_policy(const geist_hip_loss_rows &r, const geist_hip_policy &p, float *loss,
-                   float *logprob, float *entropy, void *ws, hipStream_t stream) {
-    LossArgs a     = args_of(r, ws);
+                   float *logprob, float *entropy, void *ws, int cu_count, hipStream_t stream) {
+    LossArgs a     = args_of(r, ws, cu_count);
     a.tokens       = p.d_tokens;
     a.advantage    = p.d_advantage;
     a.old_lp       = p.d_old;
@@ -183,8 +186,8 @@ void launch_policy(const geist_hip_loss_rows &r, const geist_hip_policy &p, floa
 }
 
 void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, float *loss, void *ws,
-                    hipStream_t stream) {
-    LossArgs a = args_of(r, ws);
+                    int cu_count, hipStream_t stream) {
+    LossArgs a = args_of(r, ws, cu_count);
     a.ids      = t.d_ids;
     a.values   = t.d_values;
     a.count    = t.d_count;
@@ -199,9 +202,11 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
     a.loss   = loss;
     /* ids, x, u, q of an entry, the table, and a bit per logit of a part with its head, tail and
      * alignment */
-    const size_t list   = (size_t) a.list_k * 16 + (size_t) a.slots * 4;
+    size_t       list   = (size_t) a.list_k * 16 + (size_t) a.slots * 4;
     const size_t part_n = a.chunks == 1 ? r.n_vocab : (size_t) a.chunk_vecs * (16 / elem_bytes(r.type));
     const size_t map    = a.tail ? (part_n + 64) / 32 * 4 + 4 : 0;
+    if (a.chunks == 1 && a.g)
+        list *= 2; /* the next row's is read while this one's is in use */
     if (a.chunks == 1) {
         launch_stage(r.type, STAGE_ROW, OP_DISTILL, false, a, list + map, stream);
     } else {
@@ -211,8 +216,8 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
 }
 
 void launch_preference(const geist_hip_loss_rows &r, const geist_hip_preference &p, float *loss,
-                       float *ratios, float *logprob, void *ws, hipStream_t stream) {
-    LossArgs a  = args_of(r, ws);
+                       float *ratios, float *logprob, void *ws, int cu_count, hipStream_t stream) {
+    LossArgs a  = args_of(r, ws, cu_count);
     a.coef      = r.d_grad ? reinterpret_cast<float *>(a.part + r.rows * (size_t) a.chunks) : nullptr;
     a.tokens    = p.d_tokens;
     a.ref_lp    = p.d_ref;

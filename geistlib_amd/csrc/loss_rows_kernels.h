@@ -9,21 +9,26 @@
  * with A, B, W of the row (A differs between listed and other tokens for a teacher with a tail).
  * So one streaming core serves all three: a pass that sums, a few scalars, a pass that writes.
  *
- *   k_loss_row   a workgroup per row does all of it; the row's first 16 groups of 16 bytes per thread
- *                stay in registers between the passes, so that they are read once
+ *   k_loss_row   a workgroup per row does all of it; where there is a gradient, what fits the registers
+ *                of the row stays there between the passes and is read once
  *   k_loss_sums  the sums of a part of a row (few rows; preference loss)
  *   k_loss_grad  the gradient of a part of a row from the parts' sums
+ *
+ * A row's scalars (logarithms and exponentials in binary64) and its teacher's list are the first
+ * wavefront's work alone: sixteen wavefronts that all form them cost the row 5 us of its 29.
  */
 #ifndef GEIST_LOSS_ROWS_KERNELS_H
 #define GEIST_LOSS_ROWS_KERNELS_H
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
 
 #include "loss_kernels.h"
+#include "sampler_device.h"
 
 namespace gs {
 namespace {
@@ -100,12 +105,20 @@ template <> struct Elem<GEIST_HIP_TYPE_BF16> {
 };
 
 /* ---- the workgroup -------------------------------------------------------------------------- */
-/* Orders LDS traffic only: the row's loads stay in flight across it, which __syncthreads() would wait
- * for. */
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+/* LDS writes of the own wavefront before, LDS reads behind it */
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+__device__ __forceinline__ float wave_max(float v) {
+#define GS_STEP(ctrl, rows)                                                                        \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), \
+                                                            ctrl, rows, 0xf, false)));
+    GS_STEP(0x111, 0xf) GS_STEP(0x112, 0xf) GS_STEP(0x114, 0xf) GS_STEP(0x118, 0xf)
+    GS_STEP(0x142, 0xa) GS_STEP(0x143, 0xc)
+#undef GS_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ double wave_max(double v) {
 #pragma unroll
@@ -113,41 +126,17 @@ __device__ __forceinline__ double wave_max(double v) {
         v = fmax(v, __shfl_xor(v, d));
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1)
-        v = fmaxf(v, __shfl_xor(v, d));
+/* over the workgroup, every thread gets the results; rare paths only */
+template <int THREADS, bool MAX> __device__ __forceinline__ double block_reduce(double v, double *slot) {
+    v = MAX ? wave_max(v) : wave_sum_f64(v);
+    lds_barrier();
+    if ((threadIdx.x & 63) == 0)
+        slot[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = slot[0];
+    for (int w = 1; w < THREADS / 64; ++w)
+        v = MAX ? fmax(v, slot[w]) : v + slot[w];
     return v;
-}
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1)
-        v += __shfl_xor(v, d);
-    return v;
-}
-constexpr int SLOTS = 16 * 4; /* doubles of LDS the reductions use: four per wavefront */
-/* over the workgroup; every thread gets the results */
-template <int THREADS, int K, bool MAX> __device__ __forceinline__ void block_reduce(double (&v)[K], double *slot) {
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-        v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
-    if constexpr (THREADS > 64) {
-        lds_barrier();
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int i = 0; i < K; ++i)
-                slot[(threadIdx.x >> 6) * 4 + i] = v[i];
-        lds_barrier();
-#pragma unroll
-        for (int i = 0; i < K; ++i) {
-            v[i] = slot[(threadIdx.x & (THREADS / 64 - 1)) * 4 + i];
-#pragma unroll
-            for (int d = THREADS / 128; d; d >>= 1) {
-                const double o = __shfl_xor(v[i], d);
-                v[i]           = MAX ? fmax(v[i], o) : v[i] + o;
-            }
-        }
-    }
 }
 
 /* ---- a row ---------------------------------------------------------------------------------- */
@@ -158,7 +147,6 @@ template <int TYPE> struct Row {
     mem            *g;
     const uint32_t *allowed;
     int             n, head, nvec; /* elements in front of the first 16-byte boundary, groups behind it */
-    bool            g_aligned;     /* the gradient's groups start on 16-byte boundaries too */
     int             v0, v1;        /* this workgroup's groups */
     bool            first, last;   /* it also takes the head / what is behind the last group */
 
@@ -171,7 +159,6 @@ template <int TYPE> struct Row {
         if (head > n)
             head = n;
         nvec      = (n - head) / N;
-        g_aligned = (((uintptr_t) (g + head)) & 15u) == 0;
         v0        = min(nvec, chunk * chunk_vecs);
         v1        = chunk == chunks - 1 ? nvec : min(nvec, v0 + chunk_vecs);
         first     = chunk == 0;
@@ -181,16 +168,22 @@ template <int TYPE> struct Row {
     __device__ __forceinline__ u32x4 load(int v) const {
         return *reinterpret_cast<const u32x4 *>(x + head + (long) v * N);
     }
-    __device__ __forceinline__ void store(int v, u32x4 d) const {
-        mem *p = g + head + (long) v * N;
-        if (g_aligned) {
-            *reinterpret_cast<u32x4 *>(p) = d;
+    /* for what is not read again and cannot have come from the cache */
+    __device__ __forceinline__ u32x4 load(int v, bool streamed) const {
+        const u32x4 *p = reinterpret_cast<const u32x4 *>(x + head + (long) v * N);
+        u32x4        d;
+        if (streamed) {
+            asm volatile(""); /* (keeps the two loads from being made one, an ordinary one) */
+            d = __builtin_nontemporal_load(p);
+            asm volatile("");
         } else {
-            const mem *e = reinterpret_cast<const mem *>(&d);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                p[i] = e[i];
+            d = *p;
         }
+        return d;
+    }
+    /* (the gradient's rows may start elsewhere within 16 bytes than the logits' do) */
+    __device__ __forceinline__ void store(int v, u32x4 d) const {
+        __builtin_memcpy(g + head + (long) v * N, &d, 16);
     }
     __device__ __forceinline__ bool may(int e) const {
         return !allowed || ((allowed[e >> 5] >> (e & 31)) & 1u);
@@ -250,6 +243,9 @@ template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const Lo
     return (double) x * (double) a.k;
 }
 
+__device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) { /* all ones or none */
+    return (uint32_t) __builtin_amdgcn_sbfe((int) bits, (unsigned) i, 1u);
+}
 /* A group's exponents u = w - c, and 2^u; `keep` (general rows): bits of the tokens that count. r: what
  * the soft-cap's slope is made of. */
 template <int TYPE, int FEAT>
@@ -280,7 +276,7 @@ __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_
     if ((FEAT & F_GENERAL) && a.bits) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t on = (uint32_t) ((int32_t) (keep << (31 - i)) >> 31);
+            const uint32_t on = bit_mask(keep, i);
             e[i]              = __uint_as_float(__float_as_uint(e[i]) & on);
             if (FEAT & F_ENTROPY)
                 u[i] = __uint_as_float(__float_as_uint(u[i]) & on);
@@ -410,7 +406,7 @@ __device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r,
 /* the groups from v0 + `from` on, read as they come */
 template <int TYPE, int FEAT, int THREADS, int U>
 __device__ __forceinline__ void sum_groups(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
-                                           int from, Acc &c) {
+                                           int from, bool streamed, Acc &c) {
     bool start = from == 0;
     for (int v = r.v0 + from + (int) threadIdx.x; v < r.v1; v += U * THREADS) {
         u32x4    raw[U];
@@ -419,7 +415,7 @@ __device__ __forceinline__ void sum_groups(const LossArgs &a, const Row<TYPE> &r
         for (int j = 0; j < U; ++j) {
             keep[j] = 0;
             if (v + j * THREADS < r.v1) {
-                raw[j]  = r.load(v + j * THREADS);
+                raw[j]  = r.load(v + j * THREADS, streamed);
                 keep[j] = keep_bits<TYPE, FEAT>(a, r, map, v + j * THREADS);
                 live |= 1u << j;
             }
@@ -464,50 +460,73 @@ __device__ __forceinline__ Sums careful_sums(const LossArgs &a, const Row<TYPE> 
         const int at = e - r.elem0() + N;
         return r.may(e) && !(map && ((map[at >> 5] >> (at & 31)) & 1u));
     };
-    double top[1] = {-FLT_MAX};
+    double top = -FLT_MAX;
     for (int e = lo + (int) threadIdx.x; e < hi; e += THREADS)
         if (counts(e))
-            top[0] = fmax(top[0], (double) capped<FEAT>(a, Elem<TYPE>::one(r.x[e])));
-    block_reduce<THREADS, 1, true>(top, slot);
-    Sums j     = {};
-    j.careful  = true;
-    j.m        = (float) top[0];
-    double v[2] = {0.0, 0.0};
+            top = fmax(top, (double) capped<FEAT>(a, Elem<TYPE>::one(r.x[e])));
+    Sums j    = {};
+    j.careful = true;
+    j.m       = (float) block_reduce<THREADS, true>(top, slot);
+    double s = 0.0, t = 0.0;
     for (int e = lo + (int) threadIdx.x; e < hi; e += THREADS)
         if (counts(e)) {
             const float u = (capped<FEAT>(a, Elem<TYPE>::one(r.x[e])) - j.m) * a.k;
             const float p = __builtin_amdgcn_exp2f(u);
-            v[0] += (double) p;
-            v[1] += (double) p * (double) fmaxf(u, -1e30f);
+            s += (double) p;
+            t += (double) p * (double) fmaxf(u, -1e30f);
         }
-    block_reduce<THREADS, 2, false>(v, slot);
-    j.s = v[0];
-    j.t = v[1];
+    j.s = block_reduce<THREADS, false>(s, slot);
+    j.t = block_reduce<THREADS, false>(t, slot);
     return j;
 }
-/* the threads' sums, joined against the largest reference among them */
+/* What the wavefronts of a workgroup tell one another. */
+struct Shared {
+    double s[16], t[16], slot[16];
+    float  c[16];
+    Sums   sums;
+    struct Coef {
+        float a;        /* 2^u_i (a + b u_i): 1 / S, 1 / T and the weight are in them */
+        float b;
+        float a_listed; /* 2^(w_j - top) a_listed - q_j q for listed tokens of a teacher */
+        float q;
+        bool  zero;     /* the row is written as zeros */
+    } coef;
+};
+/* lanes' sums, joined against the largest reference among them */
+template <int FEAT> __device__ __forceinline__ void join_lanes(float &c, double &s, double &t) {
+    const float  top = wave_max(c);
+    const float  d   = c - top; /* (NaN beside +inf: so is the row) */
+    const double sc  = (double) __builtin_amdgcn_exp2f(d);
+    if (FEAT & F_ENTROPY)
+        t = wave_sum_f64(sc * (t + (s == 0.0 ? 0.0 : s * (double) d)));
+    s = wave_sum_f64(sc * s);
+    c = top;
+}
 template <int FEAT, int THREADS>
-__device__ __forceinline__ Sums join_threads(const Acc &c, double *slot) {
-    double top[1] = {(double) c.c};
-    block_reduce<THREADS, 1, true>(top, slot);
-    Sums j = {};
-    j.c    = (float) top[0];
-    const float  d  = c.c - j.c; /* (NaN beside +inf: so is the row) */
-    const double sc = (double) __builtin_amdgcn_exp2f(d);
-    if constexpr (FEAT & F_ENTROPY) {
-        double v[2] = {sc * c.s, sc * (c.t + (c.s == 0.0 ? 0.0 : c.s * (double) d))};
-        block_reduce<THREADS, 2, false>(v, slot);
-        j.s = v[0];
-        j.t = v[1];
-    } else {
-        double v[1] = {sc * c.s};
-        block_reduce<THREADS, 1, false>(v, slot);
-        j.s = v[0];
+__device__ __forceinline__ Sums join_threads(Acc acc, Shared &sh) {
+    join_lanes<FEAT>(acc.c, acc.s, acc.t);
+    if constexpr (THREADS > 64) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0) {
+            sh.c[wave] = acc.c;
+            sh.s[wave] = acc.s;
+            sh.t[wave] = acc.t;
+        }
+        lds_barrier();
+        const bool in = lane < THREADS / 64;
+        acc.c         = in ? sh.c[lane] : C_LOW;
+        acc.s         = in ? sh.s[lane] : 0.0;
+        acc.t         = in ? sh.t[lane] : 0.0;
+        join_lanes<FEAT>(acc.c, acc.s, acc.t);
     }
+    Sums j = {};
+    j.c    = acc.c;
+    j.s    = acc.s;
+    j.t    = acc.t;
     return j;
 }
 __device__ __forceinline__ bool needs_care(const Sums &j) { return !(j.c < C_HIGH) || j.s == 0.0; }
-/* the parts of a row, joined by every wavefront for itself */
+/* the parts of a row, joined by a wavefront */
 template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p, int chunks, float k) {
     const int lane = threadIdx.x & 63;
     double    top = -INFINITY;
@@ -540,21 +559,15 @@ template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p
         if (FEAT & F_ENTROPY)
             t += sc * (p[i].t + p[i].s * d);
     }
-    j.s      = wave_sum(s);
-    j.t      = (FEAT & F_ENTROPY) ? wave_sum(t) : 0.0;
+    j.s      = wave_sum_f64(s);
+    j.t      = (FEAT & F_ENTROPY) ? wave_sum_f64(t) : 0.0;
     j.top    = p[0].top;
     j.listed = p[0].listed;
     return j;
 }
 
 /* ---- the gradient --------------------------------------------------------------------------- */
-struct Coef {
-    float a;        /* 2^u_i (a + b u_i): 1 / S, 1 / T and the weight are in them */
-    float b;
-    float a_listed; /* 2^(w_j - top) a_listed - q_j q for listed tokens of a teacher */
-    float q;
-    bool  zero;     /* the row is written as zeros */
-};
+typedef Shared::Coef Coef;
 template <int TYPE, int FEAT>
 __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32_t keep, const Coef &c,
                                             float ref) {
@@ -567,8 +580,7 @@ __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32
         if ((FEAT & F_GENERAL) && a.cap > 0.0f) /* 1 - tanh^2 = 4 (r - r^2) */
             g[i] *= 4.0f * fmaf(-r[i], r[i], r[i]);
         if ((FEAT & F_GENERAL) && a.bits) /* (a forbidden NaN has no slope either) */
-            g[i] = __uint_as_float(__float_as_uint(g[i]) &
-                                   (uint32_t) ((int32_t) (keep << (31 - i)) >> 31));
+            g[i] = __uint_as_float(__float_as_uint(g[i]) & bit_mask(keep, i));
     }
     return Elem<TYPE>::pack(g);
 }
@@ -636,30 +648,26 @@ __device__ __forceinline__ void write_rare(const LossArgs &a, const Row<TYPE> &r
 /* ---- one token per row ---------------------------------------------------------------------- */
 constexpr double LN2 = 0.693147180559945309417232;
 
-struct Token {
-    int    id; /* -1: none */
-    float  x;
-    double w; /* softcap(x) k; -inf where it is forbidden */
+template <int TYPE> struct Token {
+    typename Elem<TYPE>::mem x;
+    int                      id; /* -1: none */
+    uint32_t                 may;
+    /* softcap(x) k; -inf where the token is forbidden */
+    template <int FEAT> __device__ __forceinline__ double w(const LossArgs &a) const {
+        return !(may & 1u) ? -INFINITY : value64<TYPE, FEAT>(a, Elem<TYPE>::one(x));
+    }
 };
-template <int TYPE, int FEAT>
-__device__ __forceinline__ Token load_token(const LossArgs &a, const Row<TYPE> &r, int row) {
-    Token t;
-    t.id = a.tokens[row];
-    t.x  = 0.0f;
-    t.w  = 0.0;
+/* (only asked for here: what was asked for before need not have arrived) */
+template <int TYPE> __device__ __forceinline__ Token<TYPE> load_token(const LossArgs &a, const Row<TYPE> &r, int row) {
+    Token<TYPE> t = {};
+    t.id          = a.tokens[row];
     if (t.id < 0 || t.id >= r.n) {
         t.id = -1;
-    } else if (!r.may(t.id)) {
-        t.w = -INFINITY;
     } else {
-        t.x = Elem<TYPE>::one(r.x[t.id]);
-        t.w = value64<TYPE, FEAT>(a, t.x);
+        t.x   = r.x[t.id];
+        t.may = r.allowed ? r.allowed[t.id >> 5] >> (t.id & 31) : 1u;
     }
     return t;
-}
-/* log p of the token; -inf where the row gives it nothing or has no distribution */
-__device__ __forceinline__ double token_logprob(double s, double ref, double w) {
-    return s == 0.0 ? -INFINITY : (w - ref - log2(s)) * LN2;
 }
 /* Policy loss of a row from its sums; `lead`: this thread writes the row's outputs. */
 __device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has_token, double tw,
@@ -711,49 +719,48 @@ __device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has
 }
 /* the token's own element, over what stands there */
 template <int TYPE, int FEAT>
-__device__ __forceinline__ void write_token(const LossArgs &a, const Row<TYPE> &r, const Token &t,
+__device__ __forceinline__ void write_token(const LossArgs &a, const Row<TYPE> &r, const Token<TYPE> &t,
                                             const Coef &c, const Sums &j) {
-    const float u = (float) (t.w - j.ref(a.k));
+    const float u = (float) (t.template w<FEAT>(a) - j.ref(a.k));
     const float g = __builtin_amdgcn_exp2f(u) * ((FEAT & F_ENTROPY) ? fmaf(c.b, u, c.a) : c.a) - c.q;
-    r.g[t.id] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, t.x));
+    r.g[t.id] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, Elem<TYPE>::one(t.x)));
 }
 
 /* ---- a teacher's list ----------------------------------------------------------------------- */
 /* In LDS, of each entry: its id (-1: left out), x, w - top (w = softcap(x) k, top the largest of them),
- * its value, then q. `first`: a table of entries by id that keeps the first of a repeated id. */
+ * its value, then q. `first`: a table of entries by id that keeps the first of a repeated id. All of it is
+ * one wavefront's. */
 struct List {
-    int      *ids, *first;
-    float    *x, *u, *q;
-    uint32_t *map;
-    double    q_log_q, q_sum; /* sum q_j log q_j, sum q_j */
-    double    top;
-    double    q_u;            /* sum q_j (w_j - top) */
-    int       n;
+    int   *ids, *first;
+    float *x, *u, *q;
+    __device__ List(const LossArgs &a, void *lds) {
+        ids   = static_cast<int *>(lds);
+        x     = reinterpret_cast<float *>(ids + a.list_k);
+        u     = x + a.list_k;
+        q     = u + a.list_k;
+        first = reinterpret_cast<int *>(q + a.list_k);
+    }
+};
+struct ListSums {
+    double q_log_q, q_sum; /* sum q_j log q_j, sum q_j */
+    double top;
+    double q_u;            /* sum q_j (w_j - top) */
+    double listed;         /* with a tail: sum 2^(w_j - top), apart from the other tokens' sum, so that
+                            * neither mass is lost beside the other however far the two lie apart */
+    int    n;
 };
 /* row_top: the rows may hold their gradient already outside the workgroup's part; then only entries of
- * that part are looked up, against this top. */
-template <int TYPE, int FEAT, int THREADS>
-__device__ __forceinline__ List load_list(const LossArgs &a, const Row<TYPE> &r, int row, void *lds,
-                                          double *slot, bool want_map,
-                                          const double *row_top = nullptr) {
-    List l;
-    l.ids   = static_cast<int *>(lds);
-    l.x     = reinterpret_cast<float *>(l.ids + a.list_k);
-    l.u     = l.x + a.list_k;
-    l.q     = l.u + a.list_k;
-    l.first = reinterpret_cast<int *>(l.q + a.list_k);
-    l.map   = reinterpret_cast<uint32_t *>(l.first + a.slots);
-    constexpr int N = Elem<TYPE>::N;
-    int           k = a.list_k;
+ * that part are looked up, against this top. map, if given, is cleared and gets the listed tokens of the
+ * workgroup's part. Called by one whole wavefront. */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ ListSums read_list(const LossArgs &a, const Row<TYPE> &r, int row, const List &l,
+                                              uint32_t *map, const double *row_top) {
+    constexpr int N    = Elem<TYPE>::N;
+    const int     lane = threadIdx.x & 63;
+    int           k    = a.list_k;
     if (a.count)
         k = max(0, min(k, a.count[row]));
-    for (int i = threadIdx.x; i < a.slots; i += THREADS)
-        l.first[i] = -1;
-    const int span  = (r.last ? r.n : r.head + r.v1 * N) - r.elem0() + N; /* bits of the map */
-    const int words = want_map ? (span + 31) / 32 : 0;
-    for (int i = threadIdx.x; i < words; i += THREADS)
-        l.map[i] = 0u;
-    for (int j = threadIdx.x; j < k; j += THREADS) {
+    for (int j = lane; j < k; j += 64) {
         const int   id = a.ids[(long) row * a.list_ld + j];
         const float v  = a.values[(long) row * a.list_ld + j];
         const bool  ok = id >= 0 && id < r.n && v != -INFINITY && r.may(id);
@@ -761,8 +768,15 @@ __device__ __forceinline__ List load_list(const LossArgs &a, const Row<TYPE> &r,
         l.q[j]         = v;
         l.x[j]         = ok && (!row_top || r.mine(id)) ? Elem<TYPE>::one(r.x[id]) : 0.0f;
     }
-    lds_barrier();
-    for (int j = threadIdx.x; j < k; j += THREADS) {
+    for (int i = lane; i < a.slots; i += 64)
+        l.first[i] = -1;
+    if (map) {
+        const int span = (r.last ? r.n : r.head + r.v1 * N) - r.elem0() + N; /* bits */
+        for (int i = lane; i < (span + 31) / 32; i += 64)
+            map[i] = 0u;
+    }
+    wave_fence();
+    for (int j = lane; j < k; j += 64) {
         const int id = l.ids[j];
         if (id < 0)
             continue;
@@ -778,10 +792,10 @@ __device__ __forceinline__ List load_list(const LossArgs &a, const Row<TYPE> &r,
             at = (at + 1) & (uint32_t) (a.slots - 1);
         }
     }
-    lds_barrier();
-    double top[2] = {-INFINITY, -1e300};
-    bool   mine_out = false;
-    for (int j = threadIdx.x; j < k; j += THREADS) {
+    wave_fence();
+    float  v_top = -INFINITY;
+    double top   = -1e300;
+    for (int j = lane; j < k; j += 64) {
         const int id = l.ids[j];
         if (id < 0)
             continue;
@@ -789,65 +803,58 @@ __device__ __forceinline__ List load_list(const LossArgs &a, const Row<TYPE> &r,
         int      f;
         while (l.ids[f = l.first[at]] != id)
             at = (at + 1) & (uint32_t) (a.slots - 1);
-        if (f != j) {
-            mine_out = true; /* (the id stays until every thread has looked its own up) */
-            l.u[j]   = INFINITY;
-            continue;
-        }
-        const double w = value64<TYPE, FEAT>(a, l.x[j]);
-        top[0]         = fmax(top[0], (double) l.q[j]);
-        top[1]         = fmax(top[1], w);
-        l.u[j]         = 0.0f;
-        if (want_map && r.mine(id)) {
-            const int bit = id - r.elem0() + N;
-            atomicOr(&l.map[bit >> 5], 1u << (bit & 31));
-        }
-    }
-    block_reduce<THREADS, 2, true>(top, slot);
-    if (mine_out)
-        for (int j = threadIdx.x; j < k; j += THREADS)
-            if (l.u[j] == INFINITY)
-                l.ids[j] = -1;
-    l.top = row_top ? *row_top : top[1];
-    double v[3] = {0.0, 0.0, 0.0}; /* sums of e, e v, e u */
-    for (int j = threadIdx.x; j < k; j += THREADS)
-        if (l.ids[j] >= 0) {
-            const double z = a.tail ? (double) l.q[j] : ((double) l.q[j] - top[0]) * a.inv_t;
-            const double e = exp(z), u = value64<TYPE, FEAT>(a, l.x[j]) - l.top;
-            l.u[j]         = (float) u;
-            v[0] += e;
-            if (e != 0.0) {
-                v[1] += e * z;
-                v[2] += e * u;
+        l.u[j] = f == j ? 0.0f : 1.0f; /* (the id stays until every lane has looked its own up) */
+        if (f == j) {
+            top   = fmax(top, value64<TYPE, FEAT>(a, l.x[j]));
+            v_top = fmaxf(v_top, l.q[j]);
+            if (map && r.mine(id)) {
+                const int bit = id - r.elem0() + N;
+                atomicOr(&map[bit >> 5], 1u << (bit & 31));
             }
         }
-    block_reduce<THREADS, 3, false>(v, slot);
-    const double scale = a.tail || v[0] == 0.0 ? 1.0 : 1.0 / v[0];
-    for (int j = threadIdx.x; j < k; j += THREADS)
+    }
+    wave_fence();
+    v_top = wave_max(v_top);
+    ListSums z;
+    z.n   = k;
+    z.top = row_top ? *row_top : wave_max(top);
+    double e_sum = 0.0, ev = 0.0, eu = 0.0, listed = 0.0;
+    for (int j = lane; j < k; j += 64) {
+        if (l.ids[j] >= 0 && l.u[j] != 0.0f)
+            l.ids[j] = -1;
         if (l.ids[j] >= 0) {
-            const double z = a.tail ? (double) l.q[j] : ((double) l.q[j] - top[0]) * a.inv_t;
-            l.q[j]         = (float) (exp(z) * scale);
+            const double v = a.tail ? (double) l.q[j] : ((double) l.q[j] - (double) v_top) * a.inv_t;
+            const double e = exp(v), u = value64<TYPE, FEAT>(a, l.x[j]) - z.top;
+            l.u[j]         = (float) u;
+            e_sum += e;
+            if (e != 0.0) {
+                ev += e * v;
+                eu += e * u;
+            }
+            if (a.tail)
+                listed += (double) __builtin_amdgcn_exp2f((float) u);
         }
-    l.q_sum   = v[0] * scale;
-    l.q_log_q = v[1] * scale - (a.tail || v[0] == 0.0 ? 0.0 : log(v[0]));
-    l.q_u     = v[2] * scale;
-    l.n       = k;
-    lds_barrier();
-    return l;
-}
-/* sum of 2^(w_j - top) of the listed tokens: apart from the others', so that neither mass is lost
- * beside the other however far the two lie apart */
-template <int THREADS> __device__ __forceinline__ double listed_sum(const List &l, double *slot) {
-    double s[1] = {0.0};
-    for (int j = threadIdx.x; j < l.n; j += THREADS)
-        if (l.ids[j] >= 0)
-            s[0] += (double) __builtin_amdgcn_exp2f(l.u[j]);
-    block_reduce<THREADS, 1, false>(s, slot);
-    return s[0];
+    }
+    e_sum              = wave_sum_f64(e_sum);
+    ev                 = wave_sum_f64(ev);
+    eu                 = wave_sum_f64(eu);
+    const bool   plain = a.tail || e_sum == 0.0;
+    const double scale = plain ? 1.0 : 1.0 / e_sum;
+    for (int j = lane; j < k; j += 64)
+        if (l.ids[j] >= 0) {
+            const double v = a.tail ? (double) l.q[j] : ((double) l.q[j] - (double) v_top) * a.inv_t;
+            l.q[j]         = (float) (exp(v) * scale);
+        }
+    z.q_sum   = e_sum * scale;
+    z.q_log_q = ev * scale - (plain ? 0.0 : log(e_sum));
+    z.q_u     = eu * scale;
+    z.listed  = a.tail ? wave_sum_f64(listed) : 0.0;
+    wave_fence();
+    return z;
 }
 /* q_u and j.top (sum of q_j (w_j - top) and top) are handed in: the rows may have been replaced by
  * their gradient since */
-__device__ __forceinline__ Coef distill_coef(const LossArgs &a, int row, const List &l, double q_u,
+__device__ __forceinline__ Coef distill_coef(const LossArgs &a, int row, const ListSums &l, double q_u,
                                              const Sums &j, bool lead) {
     const double w   = a.weight ? (double) a.weight[row] : 1.0;
     const double ref = j.ref(a.k);
@@ -880,10 +887,11 @@ __device__ __forceinline__ Coef distill_coef(const LossArgs &a, int row, const L
         a.loss[row] = (float) loss;
     return c;
 }
-template <int TYPE, int FEAT, int THREADS>
-__device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> &r, const List &l,
+/* by the wavefront that read the list */
+template <int TYPE, int FEAT>
+__device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> &r, const List &l, int n,
                                              const Coef &c) {
-    for (int j = threadIdx.x; j < l.n; j += THREADS)
+    for (int j = threadIdx.x & 63; j < n; j += 64)
         if (l.ids[j] >= 0 && r.mine(l.ids[j])) {
             const float g = __builtin_amdgcn_exp2f(l.u[j]) * c.a_listed - l.q[j] * c.q;
             r.g[l.ids[j]] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, l.x[j]));
@@ -891,113 +899,154 @@ __device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> 
 }
 
 /* ---- kernels -------------------------------------------------------------------------------- */
-/* A row per workgroup. The loads of what registers hold are all asked for at the start and are in
- * flight while the teacher's list is read. */
-template <int OP, int FEAT> struct Held {
+/* Rows, one after the other, per workgroup. HELD groups of 16 bytes per thread are kept between the
+ * passes; while the gradient of a row is written, what it frees is filled with the next row, so that
+ * loads and stores overlap although a compute unit's registers hold one row at a time. HELD = 0: no
+ * gradient is wanted, rows are read as they come by more wavefronts. */
+template <int OP, int FEAT> struct Held { /* what 128 registers have room for */
     static constexpr int N = FEAT == (F_GENERAL | F_ENTROPY) ? 6
                              : FEAT & F_GENERAL           ? 8
-                             : OP == OP_DISTILL           ? 12
+                             : FEAT || OP == OP_DISTILL   ? 12
                                                           : 16;
 };
 constexpr int UH = 2;
-template <int TYPE, int OP, int FEAT, int THREADS>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_loss_row(LossArgs a) {
-    __shared__ double slot[SLOTS];
+/* A value the compiler knows nothing about: what is worked out of it stays inside the loop over rows,
+ * where hoisted it would take the registers the row is held in. */
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+template <int TYPE, int OP, int FEAT, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) {
+    __shared__ Shared sh;
     extern __shared__ __align__(16) char lds[];
-    constexpr int   HELD = Held<OP, FEAT>::N;
-    const int       row = blockIdx.x, tid = (int) threadIdx.x;
-    const Row<TYPE> r(a, row, 0, 1, 0);
-    u32x4           raw[HELD];
+    constexpr int H    = HELD ? HELD : 1;
+    const int     tid  = (int) threadIdx.x;
+    const bool    lead = tid < 64; /* the wavefront that forms the row's scalars */
+    const bool    tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    /* two lists (of this row and the next), then the map */
+    const int       list_bytes = OP == OP_DISTILL ? a.list_k * 16 + a.slots * 4 : 0;
+    uint32_t *const map = tail ? reinterpret_cast<uint32_t *>(lds + (HELD ? 2 : 1) * list_bytes) : nullptr;
+    int             row = blockIdx.x, turn = 0;
+    Row<TYPE>       r(a, row, 0, 1, 0);
+    ListSums        ls = {}, ls_next = {};
+    u32x4           raw[H];
+    if constexpr (OP == OP_DISTILL) {
+        if (lead) /* (in front of the row's loads: loads return in order) */
+            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), map, nullptr);
+        if (tail)
+            lds_barrier();
+    }
+    if constexpr (HELD > 0) {
 #pragma unroll
-    for (int h = 0; h < HELD; ++h)
-        if (h * THREADS + tid < r.nvec)
-            raw[h] = r.load(h * THREADS + tid);
-    List  l;
-    Token t;
-    if constexpr (OP == OP_DISTILL)
-        l = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, (FEAT & F_GENERAL) && a.tail);
-    else
-        t = load_token<TYPE, FEAT>(a, r, row);
-    const uint32_t *map = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail ? l.map : nullptr;
-    Acc acc;
+        for (int h = 0; h < HELD; ++h)
+            if (h * THREADS + tid < r.nvec)
+                raw[h] = r.load(h * THREADS + tid, a.streamed);
+    }
+    for (;;) {
+        Token<TYPE> t = {};
+        if constexpr (OP != OP_DISTILL)
+            t = load_token<TYPE>(a, r, row);
+        Acc acc;
+        if constexpr (HELD > 0) {
+            const int at = fresh(tid);
 #pragma unroll
-    for (int h = 0; h < HELD; h += UH) {
-        uint32_t keep[UH], live = 0;
-        u32x4    some[UH];
+            for (int h = 0; h < HELD; h += UH) {
+                uint32_t keep[UH], live = 0;
+                u32x4    some[UH];
 #pragma unroll
-        for (int i = 0; i < UH; ++i) {
-            const int v = (h + i) * THREADS + tid;
-            keep[i]     = 0;
-            some[i]     = raw[h + i];
-            if (v < r.nvec) {
-                keep[i] = keep_bits<TYPE, FEAT>(a, r, map, v);
-                live |= 1u << i;
+                for (int i = 0; i < UH; ++i) {
+                    const int v = (h + i) * THREADS + at;
+                    keep[i]     = 0;
+                    some[i]     = raw[h + i];
+                    if (v < r.nvec) {
+                        keep[i] = keep_bits<TYPE, FEAT>(a, r, map, v);
+                        live |= 1u << i;
+                    }
+                }
+                if (h == 0 && live)
+                    acc_move(acc, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
+                acc_batch<TYPE, FEAT, UH>(a, acc, some, keep, live);
+                __builtin_amdgcn_sched_barrier(0); /* (interleaved, the batches would not fit) */
+            }
+            sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, HELD * THREADS, false, acc);
+        } else {
+            sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, a.streamed, acc);
+        }
+        acc_loose<TYPE, FEAT>(a, r, map, acc);
+        Sums j = join_threads<FEAT, THREADS>(acc, sh);
+        if (needs_care(j))
+            j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
+        if (lead) {
+            if (!j.careful)
+                rebase(j);
+            Coef c;
+            if constexpr (OP == OP_DISTILL) {
+                j.top    = ls.top;
+                j.listed = ls.listed;
+                c        = distill_coef(a, row, ls, ls.q_u, j, tid == 0);
+            } else {
+                c = policy_coef(a, row, t.id >= 0, t.template w<FEAT>(a), j, FEAT & F_ENTROPY, tid == 0);
+            }
+            if (tid == 0) {
+                sh.sums = j;
+                sh.coef = c;
             }
         }
-        if (h == 0 && live)
-            acc_move(acc, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
-        acc_batch<TYPE, FEAT, UH>(a, acc, some, keep, live);
-        __builtin_amdgcn_sched_barrier(0); /* (interleaved, the batches would not fit the registers) */
-    }
-    sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, HELD * THREADS, acc);
-    acc_loose<TYPE, FEAT>(a, r, map, acc);
-    Sums j = join_threads<FEAT, THREADS>(acc, slot);
-    auto coef = [&]() {
-        if constexpr (OP == OP_DISTILL) {
-            j.top = l.top;
-            if (map)
-                j.listed = listed_sum<THREADS>(l, slot);
-            return distill_coef(a, row, l, l.q_u, j, tid == 0);
+        if constexpr (HELD == 0) {
+            return; /* (a workgroup per row) */
         } else {
-            return policy_coef(a, row, t.id >= 0, t.w, j, FEAT & F_ENTROPY, tid == 0);
-        }
-    };
-    auto special = [&](const Coef &c) {
-        __syncthreads();
-        if constexpr (OP == OP_DISTILL)
-            write_listed<TYPE, FEAT, THREADS>(a, r, l, c);
-        else if (tid == 0)
-            write_token<TYPE, FEAT>(a, r, t, c, j);
-    };
-    if (needs_care(j)) { /* (what registers hold of the row is dead here) */
-        j            = careful_sums<TYPE, FEAT, THREADS>(a, r, map, slot);
-        const Coef c = coef();
-        if (r.g) {
-            __syncthreads();
-            write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
-            if (!c.zero)
-                special(c);
-        }
-        return;
-    }
-    rebase(j);
-    const Coef c = coef();
-    if (!r.g)
-        return;
-    __syncthreads(); /* every value of the row has been read before any is written */
-    if (c.zero) {
-        write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
-    } else {
+            const int       next = row + (int) gridDim.x;
+            const bool      more = next < a.rows;
+            const Row<TYPE> rn(a, more ? next : row, 0, 1, 0);
+            __syncthreads(); /* every value of the row has been read before any is written */
+            j                = sh.sums;
+            const Coef c     = sh.coef;
+            turn ^= 1;
+            if constexpr (OP == OP_DISTILL) {
+                if (lead && more)
+                    ls_next = read_list<TYPE, FEAT>(a, rn, next, List(a, lds + turn * list_bytes), map, nullptr);
+            }
+            const bool rare = c.zero || j.careful;
+            if (rare)
+                write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
+            const int at = fresh(tid);
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int v = h * THREADS + tid;
-            /* (hides that this is what the sums were made of: the compiler would keep the unpacked
-             * values, twice the registers) */
-            asm volatile("" : "+v"(raw[h]));
-            if (v < r.nvec)
-                r.store(v, group_grad<TYPE, FEAT>(a, raw[h], keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c));
-            __builtin_amdgcn_sched_barrier(0);
+            for (int h = 0; h < HELD; ++h) {
+                const int v = h * THREADS + at;
+                /* (hides that this is what the sums were made of: the compiler would keep the unpacked
+                 * values, twice the registers) */
+                asm volatile("" : "+v"(raw[h]));
+                if (!rare && v < r.nvec)
+                    r.store(v, group_grad<TYPE, FEAT>(a, raw[h], keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c));
+                if (more && v < rn.nvec)
+                    raw[h] = rn.load(v, a.streamed);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!rare) {
+                write_groups<TYPE, FEAT, THREADS, 2>(a, r, c, j, HELD * THREADS);
+                write_loose<TYPE, FEAT>(a, r, c, j);
+            }
+            __syncthreads();
+            if (lead && !c.zero) {
+                if constexpr (OP == OP_DISTILL)
+                    write_listed<TYPE, FEAT>(a, r, List(a, lds + (turn ^ 1) * list_bytes), ls.n, c);
+                else if (tid == 0)
+                    write_token<TYPE, FEAT>(a, r, t, c, j);
+            }
+            if (!more)
+                return;
+            row = next;
+            r   = rn;
+            ls  = ls_next;
         }
-        write_groups<TYPE, FEAT, THREADS, 4>(a, r, c, j, HELD * THREADS);
-        write_loose<TYPE, FEAT>(a, r, c, j);
-        special(c);
     }
 }
 
 /* The sums of a part of a row. */
 template <int TYPE, int OP, int FEAT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
-    __shared__ double slot[SLOTS];
+    __shared__ Shared sh;
     extern __shared__ __align__(16) char lds[];
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     if constexpr (OP == OP_PREFERENCE) {
@@ -1006,72 +1055,84 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
     }
     const Row<TYPE> r(a, row, chunk, a.chunks, a.chunk_vecs);
     const bool      tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    const bool      lead = threadIdx.x < 64;
     Acc             acc;
-    double          at = 0.0;
-    List            l = {};
+    ListSums        ls = {};
+    Token<TYPE>     t  = {};
+    uint32_t       *map = nullptr;
     if constexpr (OP == OP_DISTILL) {
-        if (tail || chunk == 0) {
-            l  = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, tail);
-            at = l.q_u;
-        }
-    } else if (chunk == 0) {
-        at = load_token<TYPE, FEAT>(a, r, row).w;
-    }
-    const uint32_t *map = tail ? l.map : nullptr;
-    sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, acc);
-    acc_loose<TYPE, FEAT>(a, r, map, acc);
-    Sums j = join_threads<FEAT, THREADS>(acc, slot);
-    if (needs_care(j))
-        j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, slot);
-    if (OP == OP_DISTILL && chunk == 0) {
-        j.top = l.top;
         if (tail)
-            j.listed = listed_sum<THREADS>(l, slot);
+            map = reinterpret_cast<uint32_t *>(lds + a.list_k * 16 + a.slots * 4);
+        if (lead && (tail || chunk == 0))
+            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), map, nullptr);
+        if (tail)
+            lds_barrier();
+    } else if (chunk == 0) {
+        t = load_token<TYPE>(a, r, row);
     }
+    sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, row < a.streamed_rows, acc);
+    acc_loose<TYPE, FEAT>(a, r, map, acc);
+    Sums j = join_threads<FEAT, THREADS>(acc, sh);
+    if (needs_care(j))
+        j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
     if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.coef)
         a.coef[row] = 0.0f;
     if (threadIdx.x == 0)
-        a.part[(long) row * a.chunks + chunk] = {j.s, j.t, j.ref(a.k), at, j.listed, j.top, j.m, j.careful};
+        a.part[(long) row * a.chunks + chunk] = {
+            j.s, j.t, j.ref(a.k), OP == OP_DISTILL ? ls.q_u : t.template w<FEAT>(a), ls.listed, ls.top, j.m, j.careful};
 }
 
 /* The gradient of a part of a row from the parts' sums; without one, a workgroup per row writes the
  * row's outputs. */
 template <int TYPE, int OP, int FEAT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, int chunk_vecs) {
-    __shared__ double slot[SLOTS];
+    __shared__ Shared sh;
     extern __shared__ __align__(16) char lds[];
-    const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    /* the last rows first: they are the likeliest to be in the cache still */
+    const int row = a.rows - 1 - (int) (blockIdx.x / chunks), chunk = blockIdx.x % chunks;
     if constexpr (OP == OP_PREFERENCE) {
         if (row < a.seq_start[0] || row >= a.seq_start[2 * a.n_pairs])
             return;
     }
-    const LossPart *p  = a.part + (long) row * a.chunks;
-    Sums            j  = join_parts<FEAT>(p, a.chunks, a.k);
-    rebase(j);
-    const double    at = p[0].a;
     const Row<TYPE> r(a, row, chunk, chunks, chunk_vecs);
-    const bool      lead = chunk == 0 && threadIdx.x == 0;
-    List            l    = {};
-    Token           t    = {-1, 0.0f, 0.0};
-    Coef            c;
-    if constexpr (OP == OP_DISTILL) {
-        l = load_list<TYPE, FEAT, THREADS>(a, r, row, lds, slot, false, &j.top);
-        c = distill_coef(a, row, l, at, j, lead);
-    } else {
-        const int  id        = a.tokens[row];
-        const bool has_token = id >= 0 && id < a.n;
-        if (has_token && r.g && r.mine(id))
-            t = load_token<TYPE, FEAT>(a, r, row);
-        if constexpr (OP == OP_PREFERENCE) {
+    const bool      lead = threadIdx.x < 64;
+    ListSums        ls   = {};
+    Token<TYPE>     t    = {};
+    if (lead) {
+        const LossPart *p     = a.part + (long) row * a.chunks;
+        const bool      first = chunk == 0 && threadIdx.x == 0;
+        Coef            c;
+        int             id = -1;
+        if constexpr (OP != OP_DISTILL) {
+            id = a.tokens[row];
+            if (r.g && id >= 0 && id < a.n && r.mine(id))
+                t = load_token<TYPE>(a, r, row);
+            else
+                t.id = -1;
+        }
+        Sums         j  = join_parts<FEAT>(p, a.chunks, a.k);
+        const double at = p[0].a;
+        if (!j.careful)
+            rebase(j);
+        if constexpr (OP == OP_DISTILL) {
+            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), nullptr, &j.top);
+            c  = distill_coef(a, row, ls, at, j, first);
+        } else if constexpr (OP == OP_PREFERENCE) {
             const double d = (double) a.coef[row] * a.inv_t;
             c              = {(float) (-d / j.s), 0.0f, 0.0f, (float) -d, d == 0.0};
         } else {
-            c = policy_coef(a, row, has_token, at, j, FEAT & F_ENTROPY, lead);
+            c = policy_coef(a, row, id >= 0 && id < a.n, at, j, FEAT & F_ENTROPY, first);
+        }
+        if (threadIdx.x == 0) {
+            sh.sums = j;
+            sh.coef = c;
         }
     }
     if (!r.g)
         return;
-    __syncthreads(); /* the part's values have been read before any is written */
+    __syncthreads(); /* the part's special values have been read before any is written */
+    const Sums j = sh.sums;
+    const Coef c = sh.coef;
     if (c.zero || j.careful) {
         write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
     } else {
@@ -1081,10 +1142,11 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
     if (c.zero)
         return;
     __syncthreads();
-    if constexpr (OP == OP_DISTILL) {
-        write_listed<TYPE, FEAT, THREADS>(a, r, l, c);
-    } else if (threadIdx.x == 0 && t.id >= 0) {
-        write_token<TYPE, FEAT>(a, r, t, c, j);
+    if (lead) {
+        if constexpr (OP == OP_DISTILL)
+            write_listed<TYPE, FEAT>(a, r, List(a, lds), ls.n, c);
+        else if (threadIdx.x == 0 && t.id >= 0)
+            write_token<TYPE, FEAT>(a, r, t, c, j);
     }
 }
 
@@ -1092,15 +1154,20 @@ template <int TYPE, int OP, int FEAT>
 void launch_one(LossStage stage, const LossArgs &a, size_t lds, int chunks, int chunk_vecs, hipStream_t stream) {
     if (stage == STAGE_ROW) {
         if constexpr (OP != OP_PREFERENCE) {
-            const int need = a.n / Elem<TYPE>::N / Held<OP, FEAT>::N;
-            if (need <= 128)
-                k_loss_row<TYPE, OP, FEAT, 128><<<dim3(a.rows), 128, lds, stream>>>(a);
+            constexpr int H = Held<OP, FEAT>::N;
+            /* sixteen wavefronts of 128 registers fit a compute unit */
+            auto grid = [&](int threads) { return dim3(std::min(a.rows, a.cu_count * (1024 / threads))); };
+            const int need = a.n / Elem<TYPE>::N / H;
+            if (!a.g)
+                k_loss_row<TYPE, OP, FEAT, 256, 0><<<dim3(a.rows), 256, lds, stream>>>(a);
+            else if (need <= 128)
+                k_loss_row<TYPE, OP, FEAT, 128, H><<<grid(128), 128, lds, stream>>>(a);
             else if (need <= 256)
-                k_loss_row<TYPE, OP, FEAT, 256><<<dim3(a.rows), 256, lds, stream>>>(a);
+                k_loss_row<TYPE, OP, FEAT, 256, H><<<grid(256), 256, lds, stream>>>(a);
             else if (need <= 512)
-                k_loss_row<TYPE, OP, FEAT, 512><<<dim3(a.rows), 512, lds, stream>>>(a);
+                k_loss_row<TYPE, OP, FEAT, 512, H><<<grid(512), 512, lds, stream>>>(a);
             else
-                k_loss_row<TYPE, OP, FEAT, 1024><<<dim3(a.rows), 1024, lds, stream>>>(a);
+                k_loss_row<TYPE, OP, FEAT, 1024, H><<<grid(1024), 1024, lds, stream>>>(a);
         }
     } else if (stage == STAGE_SUMS) {
         k_loss_sums<TYPE, OP, FEAT, 256><<<dim3((unsigned) a.rows * a.chunks), 256, lds, stream>>>(a);
