@@ -34,7 +34,7 @@ struct LossArgs {
     float           tanh_k;  /* 2 log2(e) / cap */
     double          inv_t;
     int             chunks, chunk_vecs;
-    int             cu_count;
+    int             stash, stash_at; /* k_loss_row: groups per thread that LDS keeps, and where */
     bool            streamed;      /* the rows are too many bytes to have come from the cache */
     int             streamed_rows; /* rows of the first pass over them that will not be in it later either */
     LossPart       *part;    /* [rows][chunks] */
@@ -65,11 +65,11 @@ void launch_loss(LossStage stage, int op, int feat, const LossArgs &a, size_t ld
                  int chunk_vecs, hipStream_t stream);
 
 void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, float *loss, void *ws,
-                    int cu_count, hipStream_t stream);
+                    hipStream_t stream);
 void launch_policy(const geist_hip_loss_rows &r, const geist_hip_policy &p, float *loss,
-                   float *logprob, float *entropy, void *ws, int cu_count, hipStream_t stream);
+                   float *logprob, float *entropy, void *ws, hipStream_t stream);
 void launch_preference(const geist_hip_loss_rows &r, const geist_hip_preference &p, float *loss,
-                       float *ratios, float *logprob, void *ws, int cu_count, hipStream_t stream);
+                       float *ratios, float *logprob, void *ws, hipStream_t stream);
 
 } // namespace gs
 #endif /* GEIST_LOSS_KERNELS_H */

@@ -117,7 +117,7 @@ constexpr size_t CACHE_BYTES = (size_t) 224 << 20, KEPT_BYTES = (size_t) 160 << 
 
 size_t elem_bytes(int type) { return type == GEIST_HIP_TYPE_F32 ? 4 : 2; }
 
-LossArgs args_of(const geist_hip_loss_rows &r, void *ws, int cu_count) {
+LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
     LossArgs       a    = {};
     const LossPlan plan = loss_plan(r.rows, r.n_vocab, elem_bytes(r.type));
     a.x          = r.d_logits;
@@ -140,7 +140,6 @@ LossArgs args_of(const geist_hip_loss_rows &r, void *ws, int cu_count) {
     a.chunks     = plan.chunks;
     a.chunk_vecs = plan.chunk_vecs;
     a.part       = static_cast<LossPart *>(ws);
-    a.cu_count   = cu_count;
     const size_t row_bytes = r.ld * elem_bytes(r.type);
     a.streamed      = r.rows * row_bytes > CACHE_BYTES;
     a.streamed_rows = a.streamed ? (int) (r.d_grad ? r.rows - KEPT_BYTES / row_bytes : r.rows) : 0;
@@ -162,8 +161,8 @@ void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArg
 } // namespace
 
 void launch_policy(const geist_hip_loss_rows &r, const geist_hip_policy &p, float *loss,
-                   float *logprob, float *entropy, void *ws, int cu_count, hipStream_t stream) {
-    LossArgs a     = args_of(r, ws, cu_count);
+                   float *logprob, float *entropy, void *ws, hipStream_t stream) {
+    LossArgs a     = args_of(r, ws);
     a.tokens       = p.d_tokens;
     a.advantage    = p.d_advantage;
     a.old_lp       = p.d_old;
@@ -186,8 +185,8 @@ void launch_policy(const geist_hip_loss_rows &r, const geist_hip_policy &p, floa
 }
 
 void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, float *loss, void *ws,
-                    int cu_count, hipStream_t stream) {
-    LossArgs a = args_of(r, ws, cu_count);
+                    hipStream_t stream) {
+    LossArgs a = args_of(r, ws);
     a.ids      = t.d_ids;
     a.values   = t.d_values;
     a.count    = t.d_count;
@@ -202,11 +201,9 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
     a.loss   = loss;
     /* ids, x, u, q of an entry, the table, and a bit per logit of a part with its head, tail and
      * alignment */
-    size_t       list   = (size_t) a.list_k * 16 + (size_t) a.slots * 4;
+    const size_t list   = (size_t) a.list_k * 16 + (size_t) a.slots * 4;
     const size_t part_n = a.chunks == 1 ? r.n_vocab : (size_t) a.chunk_vecs * (16 / elem_bytes(r.type));
     const size_t map    = a.tail ? (part_n + 64) / 32 * 4 + 4 : 0;
-    if (a.chunks == 1 && a.g)
-        list *= 2; /* the next row's is read while this one's is in use */
     if (a.chunks == 1) {
         launch_stage(r.type, STAGE_ROW, OP_DISTILL, false, a, list + map, stream);
     } else {
@@ -216,8 +213,8 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
 }
 
 void launch_preference(const geist_hip_loss_rows &r, const geist_hip_preference &p, float *loss,
-                       float *ratios, float *logprob, void *ws, int cu_count, hipStream_t stream) {
-    LossArgs a  = args_of(r, ws, cu_count);
+                       float *ratios, float *logprob, void *ws, hipStream_t stream) {
+    LossArgs a  = args_of(r, ws);
     a.coef      = r.d_grad ? reinterpret_cast<float *>(a.part + r.rows * (size_t) a.chunks) : nullptr;
     a.tokens    = p.d_tokens;
     a.ref_lp    = p.d_ref;

@@ -181,20 +181,36 @@ template <int TYPE> struct Row {
         }
         return d;
     }
+    /* to the place of lane 0 in `wave`, each lane's 16 bytes behind it */
+    __device__ __forceinline__ void load_to_lds(int v, u32x4 *wave, bool streamed) const {
+        typedef const __attribute__((address_space(1))) void *global_ptr;
+        typedef __attribute__((address_space(3))) void       *lds_ptr;
+        const global_ptr p = (global_ptr) (x + head + (long) v * N);
+        const lds_ptr    l = (lds_ptr) wave;
+        if (streamed)
+            __builtin_amdgcn_global_load_lds(p, l, 16, 0, 2);
+        else
+            __builtin_amdgcn_global_load_lds(p, l, 16, 0, 0);
+    }
     /* (the gradient's rows may start elsewhere within 16 bytes than the logits' do) */
-    __device__ __forceinline__ void store(int v, u32x4 d) const {
-        __builtin_memcpy(g + head + (long) v * N, &d, 16);
+    __device__ __forceinline__ void store(int v, u32x4 d, bool streamed) const {
+        typedef u32x4 __attribute__((aligned(2))) loose_u32x4;
+        loose_u32x4 *p = reinterpret_cast<loose_u32x4 *>(g + head + (long) v * N);
+        if (streamed) {
+            asm volatile("");
+            __builtin_nontemporal_store(d, p);
+            asm volatile("");
+        } else {
+            *p = d;
+        }
     }
     __device__ __forceinline__ bool may(int e) const {
         return !allowed || ((allowed[e >> 5] >> (e & 31)) & 1u);
     }
-    /* mask bits of the group that starts at element e */
+    /* mask bits of the group that starts at element e: they lie in one byte or two */
     __device__ __forceinline__ uint32_t bits(int e) const {
-        const int sh = e & 31;
-        uint32_t  w  = allowed[e >> 5] >> sh;
-        if (sh > 32 - N)
-            w |= allowed[(e >> 5) + 1] << (32 - sh);
-        return w;
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(allowed);
+        return ((uint32_t) p[e >> 3] | (uint32_t) p[(e + N - 1) >> 3] << 8) >> (e & 7);
     }
     /* the i-th element that belongs to no group: the head, then the tail; -1 behind them */
     __device__ __forceinline__ int loose(int i) const {
@@ -306,6 +322,32 @@ __device__ __forceinline__ uint32_t keep_bits(const LossArgs &a, const Row<TYPE>
     }
     return keep;
 }
+/* The allowed tokens of the groups that a thread holds, eight bits each, read once for both passes. */
+template <int TYPE, int FEAT, int THREADS, int HELD> struct HeldBits {
+    static constexpr int WORDS = FEAT & F_GENERAL ? (HELD + 3) / 4 : 1;
+    uint32_t             w[WORDS];
+    __device__ __forceinline__ void read(const LossArgs &a, const Row<TYPE> &r) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+            w[i] = ~0u;
+        if constexpr (FEAT & F_GENERAL) {
+            if (r.allowed) {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i)
+                    w[i] = 0u;
+#pragma unroll
+                for (int h = 0; h < HELD; ++h) {
+                    const int v = h * THREADS + (int) threadIdx.x;
+                    if (v < r.nvec)
+                        w[h >> 2] |= (r.bits(r.head + v * Elem<TYPE>::N) & 0xffu) << (8 * (h & 3));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t of(int h) const {
+        return FEAT & F_GENERAL ? w[h >> 2] >> (8 * (h & 3)) : ~0u;
+    }
+};
 
 /* ---- the pass that sums --------------------------------------------------------------------- */
 /* A thread sums 2^(w - c) against a reference c of its own, the largest w of its first group: later
@@ -617,7 +659,7 @@ __device__ __forceinline__ void write_groups(const LossArgs &a, const Row<TYPE> 
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (v + i * THREADS < r.v1)
-                r.store(v + i * THREADS, group_grad<TYPE, FEAT>(a, raw[i], keep[i], c, j.c));
+                r.store(v + i * THREADS, group_grad<TYPE, FEAT>(a, raw[i], keep[i], c, j.c), a.streamed);
     }
 }
 template <int TYPE, int FEAT>
@@ -634,7 +676,7 @@ template <int TYPE, int FEAT, int THREADS>
 __device__ __forceinline__ void write_rare(const LossArgs &a, const Row<TYPE> &r, const Coef &c, const Sums &j) {
     if (c.zero) {
         for (int v = r.v0 + (int) threadIdx.x; v < r.v1; v += THREADS)
-            r.store(v, u32x4{0, 0, 0, 0});
+            r.store(v, u32x4{0, 0, 0, 0}, a.streamed);
         const int e = threadIdx.x < 2 * Elem<TYPE>::N ? r.loose((int) threadIdx.x) : -1;
         if (e >= 0)
             r.g[e] = Elem<TYPE>::round(0.0f);
@@ -899,146 +941,146 @@ __device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> 
 }
 
 /* ---- kernels -------------------------------------------------------------------------------- */
-/* Rows, one after the other, per workgroup. HELD groups of 16 bytes per thread are kept between the
- * passes; while the gradient of a row is written, what it frees is filled with the next row, so that
- * loads and stores overlap although a compute unit's registers hold one row at a time. HELD = 0: no
- * gradient is wanted, rows are read as they come by more wavefronts. */
-template <int OP, int FEAT> struct Held { /* what 128 registers have room for */
-    static constexpr int N = FEAT == (F_GENERAL | F_ENTROPY) ? 6
-                             : FEAT & F_GENERAL           ? 8
-                             : FEAT || OP == OP_DISTILL   ? 12
-                                                          : 16;
+/* A workgroup per row. HELD groups of 16 bytes per thread are kept between the passes: all of them are
+ * asked for at the start, and the gradient goes out in one go (reading and writing in turn moves 5.8 TB/s
+ * on this pattern, a next row's loads between the stores 5.2). Longer rows have further groups loaded
+ * straight into LDS (a.stash per thread), and what is left is read twice. HELD = 0: no gradient is wanted, the row
+ * is read as it comes by more wavefronts. */
+template <int TYPE, int OP, int FEAT> struct Held { /* what 128 registers have room for */
+    static constexpr int N = TYPE == GEIST_HIP_TYPE_F32        ? (FEAT & F_GENERAL ? 12 : 16)
+                             : FEAT == (F_GENERAL | F_ENTROPY) ? 4
+                             : FEAT & F_GENERAL                ? 8
+                             : OP == OP_DISTILL                ? 12
+                                                               : 16;
 };
 constexpr int UH = 2;
-/* A value the compiler knows nothing about: what is worked out of it stays inside the loop over rows,
- * where hoisted it would take the registers the row is held in. */
-__device__ __forceinline__ int fresh(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
 template <int TYPE, int OP, int FEAT, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) {
     __shared__ Shared sh;
     extern __shared__ __align__(16) char lds[];
-    constexpr int H    = HELD ? HELD : 1;
-    const int     tid  = (int) threadIdx.x;
-    const bool    lead = tid < 64; /* the wavefront that forms the row's scalars */
-    const bool    tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
-    /* two lists (of this row and the next), then the map */
-    const int       list_bytes = OP == OP_DISTILL ? a.list_k * 16 + a.slots * 4 : 0;
-    uint32_t *const map = tail ? reinterpret_cast<uint32_t *>(lds + (HELD ? 2 : 1) * list_bytes) : nullptr;
-    int             row = blockIdx.x, turn = 0;
-    Row<TYPE>       r(a, row, 0, 1, 0);
-    ListSums        ls = {}, ls_next = {};
-    u32x4           raw[H];
+    const int       row = blockIdx.x, tid = (int) threadIdx.x;
+    const bool      lead = tid < 64; /* the wavefront that forms the row's scalars */
+    const bool      tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    const Row<TYPE> r(a, row, 0, 1, 0);
+    uint32_t       *map = nullptr;
+    ListSums        ls  = {};
+    Token<TYPE>     t   = {};
     if constexpr (OP == OP_DISTILL) {
-        if (lead) /* (in front of the row's loads: loads return in order) */
-            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), map, nullptr);
         if (tail)
-            lds_barrier();
+            map = reinterpret_cast<uint32_t *>(lds + a.list_k * 16 + a.slots * 4);
+        if (lead) /* (in front of its loads of the row: loads return in order) */
+            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), map, nullptr);
     }
+    Acc   acc;
+    u32x4 raw[HELD ? HELD : 1];
     if constexpr (HELD > 0) {
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
             if (h * THREADS + tid < r.nvec)
                 raw[h] = r.load(h * THREADS + tid, a.streamed);
     }
-    for (;;) {
-        Token<TYPE> t = {};
-        if constexpr (OP != OP_DISTILL)
-            t = load_token<TYPE>(a, r, row);
-        Acc acc;
-        if constexpr (HELD > 0) {
-            const int at = fresh(tid);
+    /* [stash][THREADS] groups, each the own thread's */
+    u32x4 *const stash = reinterpret_cast<u32x4 *>(lds + a.stash_at);
+    if constexpr (HELD > 0)
+        for (int h = 0; h < a.stash; ++h)
+            if ((HELD + h) * THREADS + tid < r.nvec)
+                r.load_to_lds((HELD + h) * THREADS + tid, stash + h * THREADS + (tid & ~63), a.streamed);
+    HeldBits<TYPE, FEAT, THREADS, HELD ? HELD : 1> bits;
+    if constexpr (OP != OP_DISTILL)
+        t = load_token<TYPE>(a, r, row);
+    if constexpr (HELD > 0)
+        bits.read(a, r);
+    if (tail)
+        lds_barrier();
+    if constexpr (HELD > 0) {
 #pragma unroll
-            for (int h = 0; h < HELD; h += UH) {
-                uint32_t keep[UH], live = 0;
-                u32x4    some[UH];
+        for (int h = 0; h < HELD; h += UH) {
+            uint32_t keep[UH], live = 0;
+            u32x4    some[UH];
 #pragma unroll
-                for (int i = 0; i < UH; ++i) {
-                    const int v = (h + i) * THREADS + at;
-                    keep[i]     = 0;
-                    some[i]     = raw[h + i];
-                    if (v < r.nvec) {
-                        keep[i] = keep_bits<TYPE, FEAT>(a, r, map, v);
-                        live |= 1u << i;
-                    }
+            for (int i = 0; i < UH; ++i) {
+                const int v = (h + i) * THREADS + tid;
+                keep[i]     = 0;
+                some[i]     = raw[h + i];
+                if (v < r.nvec) {
+                    keep[i] = bits.of(h + i);
+                    if ((FEAT & F_GENERAL) && map)
+                        keep[i] &= ~listed_bits<Elem<TYPE>::N>(map, v);
+                    live |= 1u << i;
                 }
-                if (h == 0 && live)
-                    acc_move(acc, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
-                acc_batch<TYPE, FEAT, UH>(a, acc, some, keep, live);
-                __builtin_amdgcn_sched_barrier(0); /* (interleaved, the batches would not fit) */
             }
-            sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, HELD * THREADS, false, acc);
-        } else {
-            sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, a.streamed, acc);
+            if (h == 0 && live)
+                acc_move(acc, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
+            acc_batch<TYPE, FEAT, UH>(a, acc, some, keep, live);
+            __builtin_amdgcn_sched_barrier(0); /* (interleaved, the batches would not fit the registers) */
         }
-        acc_loose<TYPE, FEAT>(a, r, map, acc);
-        Sums j = join_threads<FEAT, THREADS>(acc, sh);
-        if (needs_care(j))
-            j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
-        if (lead) {
-            if (!j.careful)
-                rebase(j);
-            Coef c;
-            if constexpr (OP == OP_DISTILL) {
-                j.top    = ls.top;
-                j.listed = ls.listed;
-                c        = distill_coef(a, row, ls, ls.q_u, j, tid == 0);
-            } else {
-                c = policy_coef(a, row, t.id >= 0, t.template w<FEAT>(a), j, FEAT & F_ENTROPY, tid == 0);
-            }
-            if (tid == 0) {
-                sh.sums = j;
-                sh.coef = c;
+        if (a.stash) /* what this wavefront asked for has arrived in LDS */
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int h = 0; h < a.stash; ++h) {
+            const int v = (HELD + h) * THREADS + tid;
+            if (v < r.nvec) {
+                const u32x4    one[1]  = {stash[h * THREADS + tid]};
+                const uint32_t keep[1] = {keep_bits<TYPE, FEAT>(a, r, map, v)};
+                acc_batch<TYPE, FEAT, 1>(a, acc, one, keep, 1u);
             }
         }
-        if constexpr (HELD == 0) {
-            return; /* (a workgroup per row) */
+        sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, (HELD + a.stash) * THREADS, false, acc);
+    } else {
+        sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, a.streamed, acc);
+    }
+    acc_loose<TYPE, FEAT>(a, r, map, acc);
+    Sums j = join_threads<FEAT, THREADS>(acc, sh);
+    if (needs_care(j))
+        j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
+    if (lead) {
+        if (!j.careful)
+            rebase(j);
+        Coef c;
+        if constexpr (OP == OP_DISTILL) {
+            j.top    = ls.top;
+            j.listed = ls.listed;
+            c        = distill_coef(a, row, ls, ls.q_u, j, tid == 0);
         } else {
-            const int       next = row + (int) gridDim.x;
-            const bool      more = next < a.rows;
-            const Row<TYPE> rn(a, more ? next : row, 0, 1, 0);
-            __syncthreads(); /* every value of the row has been read before any is written */
-            j                = sh.sums;
-            const Coef c     = sh.coef;
-            turn ^= 1;
-            if constexpr (OP == OP_DISTILL) {
-                if (lead && more)
-                    ls_next = read_list<TYPE, FEAT>(a, rn, next, List(a, lds + turn * list_bytes), map, nullptr);
-            }
-            const bool rare = c.zero || j.careful;
-            if (rare)
-                write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
-            const int at = fresh(tid);
+            c = policy_coef(a, row, t.id >= 0, t.template w<FEAT>(a), j, FEAT & F_ENTROPY, tid == 0);
+        }
+        if (tid == 0) {
+            sh.sums = j;
+            sh.coef = c;
+        }
+    }
+    if constexpr (HELD > 0) {
+        __syncthreads(); /* every value of the row has been read before any is written */
+        j            = sh.sums;
+        const Coef c = sh.coef;
+        if (c.zero || j.careful) {
+            write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
+        } else {
 #pragma unroll
             for (int h = 0; h < HELD; ++h) {
-                const int v = h * THREADS + at;
+                const int v = h * THREADS + tid;
                 /* (hides that this is what the sums were made of: the compiler would keep the unpacked
                  * values, twice the registers) */
                 asm volatile("" : "+v"(raw[h]));
-                if (!rare && v < r.nvec)
-                    r.store(v, group_grad<TYPE, FEAT>(a, raw[h], keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c));
-                if (more && v < rn.nvec)
-                    raw[h] = rn.load(v, a.streamed);
+                if (v < r.nvec)
+                    r.store(v, group_grad<TYPE, FEAT>(a, raw[h], bits.of(h), c, j.c), a.streamed);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (!rare) {
-                write_groups<TYPE, FEAT, THREADS, 2>(a, r, c, j, HELD * THREADS);
-                write_loose<TYPE, FEAT>(a, r, c, j);
+            for (int h = 0; h < a.stash; ++h) {
+                const int v = (HELD + h) * THREADS + tid;
+                if (v < r.nvec)
+                    r.store(v, group_grad<TYPE, FEAT>(a, stash[h * THREADS + tid],
+                                                      keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c),
+                            a.streamed);
             }
-            __syncthreads();
-            if (lead && !c.zero) {
-                if constexpr (OP == OP_DISTILL)
-                    write_listed<TYPE, FEAT>(a, r, List(a, lds + (turn ^ 1) * list_bytes), ls.n, c);
-                else if (tid == 0)
-                    write_token<TYPE, FEAT>(a, r, t, c, j);
-            }
-            if (!more)
-                return;
-            row = next;
-            r   = rn;
-            ls  = ls_next;
+            write_groups<TYPE, FEAT, THREADS, 2>(a, r, c, j, (HELD + a.stash) * THREADS);
+            write_loose<TYPE, FEAT>(a, r, c, j);
+        }
+        __syncthreads();
+        if (lead && !c.zero) {
+            if constexpr (OP == OP_DISTILL)
+                write_listed<TYPE, FEAT>(a, r, List(a, lds), ls.n, c);
+            else if (tid == 0 && t.id >= 0)
+                write_token<TYPE, FEAT>(a, r, t, c, j);
         }
     }
 }
@@ -1150,24 +1192,38 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
     }
 }
 
+constexpr int LDS_MOST = 158 * 1024; /* of 160 KB; the rest is what a kernel declares itself */
+static_assert(sizeof(Shared) <= 2048, "beside the dynamic part");
+
 template <int TYPE, int OP, int FEAT>
 void launch_one(LossStage stage, const LossArgs &a, size_t lds, int chunks, int chunk_vecs, hipStream_t stream) {
     if (stage == STAGE_ROW) {
         if constexpr (OP != OP_PREFERENCE) {
-            constexpr int H = Held<OP, FEAT>::N;
-            /* sixteen wavefronts of 128 registers fit a compute unit */
-            auto grid = [&](int threads) { return dim3(std::min(a.rows, a.cu_count * (1024 / threads))); };
-            const int need = a.n / Elem<TYPE>::N / H;
-            if (!a.g)
+            constexpr int H    = Held<TYPE, OP, FEAT>::N;
+            const int     vecs = a.n / Elem<TYPE>::N, need = vecs / H;
+            if (!a.g) {
                 k_loss_row<TYPE, OP, FEAT, 256, 0><<<dim3(a.rows), 256, lds, stream>>>(a);
-            else if (need <= 128)
-                k_loss_row<TYPE, OP, FEAT, 128, H><<<grid(128), 128, lds, stream>>>(a);
-            else if (need <= 256)
-                k_loss_row<TYPE, OP, FEAT, 256, H><<<grid(256), 256, lds, stream>>>(a);
-            else if (need <= 512)
-                k_loss_row<TYPE, OP, FEAT, 512, H><<<grid(512), 512, lds, stream>>>(a);
-            else
-                k_loss_row<TYPE, OP, FEAT, 1024, H><<<grid(1024), 1024, lds, stream>>>(a);
+            } else if (need <= 128) {
+                k_loss_row<TYPE, OP, FEAT, 128, H><<<dim3(a.rows), 128, lds, stream>>>(a);
+            } else if (need <= 256) {
+                k_loss_row<TYPE, OP, FEAT, 256, H><<<dim3(a.rows), 256, lds, stream>>>(a);
+            } else if (need <= 512) {
+                k_loss_row<TYPE, OP, FEAT, 512, H><<<dim3(a.rows), 512, lds, stream>>>(a);
+            } else {
+                /* one workgroup to a compute unit: all of its LDS is free for the row */
+                LossArgs  b    = a;
+                const int most = (LDS_MOST - (int) ((lds + 15) / 16 * 16)) / (1024 * 16);
+                b.stash        = std::max(0, std::min(most, vecs / 1024 + 1 - H));
+                b.stash_at     = (int) ((lds + 15) / 16 * 16);
+                const size_t all = (size_t) b.stash_at + (size_t) b.stash * 1024 * 16;
+                auto        *k   = k_loss_row<TYPE, OP, FEAT, 1024, H>;
+                /* (more than a launch gets unasked; where it is refused so is the launch, which the caller
+                 * sees) */
+                if (all > 64 * 1024)
+                    (void) hipFuncSetAttribute(reinterpret_cast<const void *>(k),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MOST);
+                k<<<dim3(a.rows), 1024, all, stream>>>(b);
+            }
         }
     } else if (stage == STAGE_SUMS) {
         k_loss_sums<TYPE, OP, FEAT, 256><<<dim3((unsigned) a.rows * a.chunks), 256, lds, stream>>>(a);

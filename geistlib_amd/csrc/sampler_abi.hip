@@ -2563,7 +2563,7 @@ int geist_hip_distill_rows(geist_hip_sampler *s, const struct geist_hip_loss_row
     if (rc != GEIST_HIP_OK)
         return fail(s, rc, "distillation loss: %s", why.text);
     HIPCHK(s, hipSetDevice(s->device));
-    launch_distill(*rows, *teacher, d_loss, d_workspace, s->cu_count, s->stream);
+    launch_distill(*rows, *teacher, d_loss, d_workspace, s->stream);
     return after_launch(s, "distillation loss");
 }
 
@@ -2580,7 +2580,7 @@ int geist_hip_policy_loss_rows(geist_hip_sampler *s, const struct geist_hip_loss
     if (rc != GEIST_HIP_OK)
         return fail(s, rc, "policy loss: %s", why.text);
     HIPCHK(s, hipSetDevice(s->device));
-    launch_policy(*rows, *policy, d_loss, d_logprob, d_entropy, d_workspace, s->cu_count, s->stream);
+    launch_policy(*rows, *policy, d_loss, d_logprob, d_entropy, d_workspace, s->stream);
     return after_launch(s, "policy loss");
 }
 
@@ -2597,7 +2597,7 @@ int geist_hip_preference_loss(geist_hip_sampler *s, const struct geist_hip_loss_
     if (rc != GEIST_HIP_OK)
         return fail(s, rc, "preference loss: %s", why.text);
     HIPCHK(s, hipSetDevice(s->device));
-    launch_preference(*rows, *preference, d_loss, d_ratios, d_logprob, d_workspace, s->cu_count, s->stream);
+    launch_preference(*rows, *preference, d_loss, d_ratios, d_logprob, d_workspace, s->stream);
     return after_launch(s, "preference loss");
 }
 
