@@ -13,7 +13,8 @@ namespace gs {
 
 /* FEAT bits: what a kernel is compiled for beyond plain rows */
 constexpr int F_ENTROPY = 1; /* sum 2^u u, and a term of p_i u_i in the gradient */
-constexpr int F_GENERAL = 2; /* soft-cap, allowed-token mask or a teacher's tail, looked at per group */
+constexpr int F_CAP     = 2; /* a soft-cap */
+constexpr int F_BITS    = 4; /* an allowed-token mask or a teacher's tail: tokens that do not count */
 
 constexpr int OP_TOKEN      = 0; /* one token per row, policy loss */
 constexpr int OP_DISTILL    = 1;
@@ -26,7 +27,6 @@ struct LossArgs {
     int             n, rows;
     const uint32_t *allowed;
     long            allowed_ld;
-    int             bits;    /* there is a mask or a tail */
     float           k;       /* log2(e) / T */
     float           cap;     /* 0 = none */
     float           inv_cap;

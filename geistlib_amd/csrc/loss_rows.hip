@@ -128,7 +128,6 @@ LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
     a.rows       = (int) r.rows;
     a.allowed    = r.d_allowed;
     a.allowed_ld = (long) r.allowed_ld;
-    a.bits       = r.d_allowed != nullptr;
     a.k          = (float) (LOG2E / (double) r.temperature);
     a.cap        = r.logit_softcap;
     if (a.cap > 0.0f) {
@@ -147,7 +146,9 @@ LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
 }
 void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArgs &a, size_t lds,
                   hipStream_t stream) {
-    const int feat = (entropy ? F_ENTROPY : 0) | (a.cap > 0.0f || a.bits ? F_GENERAL : 0);
+    const int rows = (a.cap > 0.0f ? F_CAP : 0) | (a.allowed || a.tail ? F_BITS : 0);
+    entropy        = entropy || (op == OP_TOKEN && rows == (F_CAP | F_BITS));
+    const int feat = rows | (entropy ? F_ENTROPY : 0);
     /* without a gradient the second launch only writes the rows' outputs */
     const int c = a.g ? a.chunks : 1, v = a.g ? a.chunk_vecs : INT32_MAX / 64;
     if (type == GEIST_HIP_TYPE_F32)
@@ -196,7 +197,6 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
     while (a.slots < 2 * a.list_k)
         a.slots *= 2;
     a.tail   = t.tail != 0;
-    a.bits   = a.bits || a.tail;
     a.weight = t.d_weight;
     a.loss   = loss;
     /* ids, x, u, q of an entry, the table, and a bit per logit of a part with its head, tail and

@@ -249,11 +249,11 @@ __device__ __forceinline__ float accurate_tanh(const LossArgs &a, float x, float
 }
 /* softcap(x) in binary32, as the degenerate rows' pass needs it */
 template <int FEAT> __device__ __forceinline__ float capped(const LossArgs &a, float x) {
-    return (FEAT & F_GENERAL) && a.cap > 0.0f ? a.cap * accurate_tanh(a, x, cap_recip(a, x)) : x;
+    return FEAT & F_CAP ? a.cap * accurate_tanh(a, x, cap_recip(a, x)) : x;
 }
 /* softcap(x) k in binary64, for the few values a row's scalars are made of */
 template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const LossArgs &a, float x) {
-    if ((FEAT & F_GENERAL) && a.cap > 0.0f)
+    if (FEAT & F_CAP)
         return (TYPE == GEIST_HIP_TYPE_F32 ? (double) a.cap * (double) a.k : (double) a.cap_k) *
                tanh((double) x / (double) a.cap);
     return (double) x * (double) a.k;
@@ -262,7 +262,7 @@ template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const Lo
 __device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) { /* all ones or none */
     return (uint32_t) __builtin_amdgcn_sbfe((int) bits, (unsigned) i, 1u);
 }
-/* A group's exponents u = w - c, and 2^u; `keep` (general rows): bits of the tokens that count. r: what
+/* A group's exponents u = w - c, and 2^u; `keep` (masked rows, tails): bits of the tokens that count. r: what
  * the soft-cap's slope is made of. */
 template <int TYPE, int FEAT>
 __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_t keep, float c,
@@ -271,7 +271,7 @@ __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_
     constexpr int N = Elem<TYPE>::N;
     float         x[N];
     Elem<TYPE>::unpack(raw, x);
-    if ((FEAT & F_GENERAL) && a.cap > 0.0f) {
+    if (FEAT & F_CAP) {
         const float at = a.cap_k - c;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -289,7 +289,7 @@ __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_
 #pragma unroll
     for (int i = 0; i < N; ++i)
         e[i] = __builtin_amdgcn_exp2f(u[i]);
-    if ((FEAT & F_GENERAL) && a.bits) {
+    if (FEAT & F_BITS) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t on = bit_mask(keep, i);
@@ -314,7 +314,7 @@ template <int TYPE, int FEAT>
 __device__ __forceinline__ uint32_t keep_bits(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
                                               int v) {
     uint32_t keep = ~0u;
-    if ((FEAT & F_GENERAL) && a.bits) {
+    if (FEAT & F_BITS) {
         if (r.allowed)
             keep = r.bits(r.head + v * Elem<TYPE>::N);
         if (map)
@@ -324,13 +324,13 @@ __device__ __forceinline__ uint32_t keep_bits(const LossArgs &a, const Row<TYPE>
 }
 /* The allowed tokens of the groups that a thread holds, eight bits each, read once for both passes. */
 template <int TYPE, int FEAT, int THREADS, int HELD> struct HeldBits {
-    static constexpr int WORDS = FEAT & F_GENERAL ? (HELD + 3) / 4 : 1;
+    static constexpr int WORDS = FEAT & F_BITS ? (HELD + 3) / 4 : 1;
     uint32_t             w[WORDS];
     __device__ __forceinline__ void read(const LossArgs &a, const Row<TYPE> &r) {
 #pragma unroll
         for (int i = 0; i < WORDS; ++i)
             w[i] = ~0u;
-        if constexpr (FEAT & F_GENERAL) {
+        if constexpr (FEAT & F_BITS) {
             if (r.allowed) {
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i)
@@ -345,7 +345,7 @@ template <int TYPE, int FEAT, int THREADS, int HELD> struct HeldBits {
         }
     }
     __device__ __forceinline__ uint32_t of(int h) const {
-        return FEAT & F_GENERAL ? w[h >> 2] >> (8 * (h & 3)) : ~0u;
+        return FEAT & F_BITS ? w[h >> 2] >> (8 * (h & 3)) : ~0u;
     }
 };
 
@@ -371,7 +371,7 @@ __device__ __forceinline__ float group_top(const LossArgs &a, u32x4 raw, uint32_
     Elem<TYPE>::unpack(raw, x);
 #pragma unroll
     for (int i = 0; i < Elem<TYPE>::N; ++i)
-        if (!(FEAT & F_GENERAL) || ((keep >> i) & 1u))
+        if (!(FEAT & F_BITS) || ((keep >> i) & 1u))
             top = fmaxf(top, x[i]);
     return capped<FEAT>(a, top); /* (it is monotone) */
 }
@@ -383,50 +383,57 @@ __device__ __forceinline__ void acc_move(Acc &c, float top, float k) {
     c.s *= sc;
     c.c = w;
 }
-/* COUNT groups, of which the j-th counts if live has bit j */
+/* the sums of COUNT groups, of which the j-th counts if live has bit j, against c */
 template <int TYPE, int FEAT, int COUNT>
-__device__ __forceinline__ void acc_batch(const LossArgs &a, Acc &c, const u32x4 (&raw)[COUNT],
-                                          const uint32_t (&keep)[COUNT], uint32_t live) {
+__device__ __forceinline__ float batch_sum(const LossArgs &a, float c, const u32x4 (&raw)[COUNT],
+                                           const uint32_t (&keep)[COUNT], uint32_t live, float &t) {
     constexpr int N = Elem<TYPE>::N;
-    for (int tries = 0; tries < 2; ++tries) {
-        float s[COUNT], t = 0.0f;
+    float         s[COUNT];
+    t = 0.0f;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            s[j] = 0.0f;
-            if ((live >> j) & 1u) {
-                float e[N], u[N], r[N];
-                group_exps<TYPE, FEAT>(a, raw[j], keep[j], c.c, e, u, r);
-                if (FEAT & F_ENTROPY) {
+    for (int j = 0; j < COUNT; ++j) {
+        s[j] = 0.0f;
+        if ((live >> j) & 1u) {
+            float e[N], u[N], r[N];
+            group_exps<TYPE, FEAT>(a, raw[j], keep[j], c, e, u, r);
+            if (FEAT & F_ENTROPY) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        t = fmaf(e[i], u[i], t);
-                }
-#pragma unroll
-                for (int half = N / 2; half; half >>= 1)
-#pragma unroll
-                    for (int i = 0; i < half; ++i)
-                        e[i] += e[i + half];
-                s[j] = e[0];
+                for (int i = 0; i < N; ++i)
+                    t = fmaf(e[i], u[i], t);
             }
-        }
 #pragma unroll
-        for (int half = COUNT / 2; half; half >>= 1)
+            for (int half = N / 2; half; half >>= 1)
 #pragma unroll
-            for (int j = 0; j < half; ++j)
-                s[j] += s[j + half];
-        if (s[0] < BATCH_HIGH || tries == 1) {
-            c.s += (double) s[0];
-            if (FEAT & F_ENTROPY)
-                c.t += (double) t;
-            break;
+                for (int i = 0; i < half; ++i)
+                    e[i] += e[i + half];
+            s[j] = e[0];
         }
+    }
+#pragma unroll
+    for (int half = COUNT / 2; half; half >>= 1)
+#pragma unroll
+        for (int j = 0; j < half; ++j)
+            s[j] += s[j + half];
+    return s[0];
+}
+template <int TYPE, int FEAT, int COUNT>
+__device__ __forceinline__ void acc_batch(const LossArgs &a, Acc &c, u32x4 (&raw)[COUNT],
+                                          const uint32_t (&keep)[COUNT], uint32_t live) {
+    float t, s = batch_sum<TYPE, FEAT, COUNT>(a, c.c, raw, keep, live, t);
+    if (__builtin_expect(!(s < BATCH_HIGH), 0)) {
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
+        for (int j = 0; j < COUNT; ++j) {
+            asm volatile("" : "+v"(raw[j])); /* (nothing is kept in registers for this case) */
             if ((live >> j) & 1u)
                 top = fmaxf(top, group_top<TYPE, FEAT>(a, raw[j], keep[j]));
+        }
         acc_move(c, top, a.k);
+        s = batch_sum<TYPE, FEAT, COUNT>(a, c.c, raw, keep, live, t);
     }
+    c.s += (double) s;
+    if (FEAT & F_ENTROPY)
+        c.t += (double) t;
 }
 template <int TYPE, int FEAT>
 __device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
@@ -619,15 +626,15 @@ __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         g[i] = e[i] * ((FEAT & F_ENTROPY) ? fmaf(c.b, u[i], c.a) : c.a);
-        if ((FEAT & F_GENERAL) && a.cap > 0.0f) /* 1 - tanh^2 = 4 (r - r^2) */
+        if (FEAT & F_CAP) /* 1 - tanh^2 = 4 (r - r^2) */
             g[i] *= 4.0f * fmaf(-r[i], r[i], r[i]);
-        if ((FEAT & F_GENERAL) && a.bits) /* (a forbidden NaN has no slope either) */
+        if (FEAT & F_BITS) /* (a forbidden NaN has no slope either) */
             g[i] = __uint_as_float(__float_as_uint(g[i]) & bit_mask(keep, i));
     }
     return Elem<TYPE>::pack(g);
 }
 template <int FEAT> __device__ __forceinline__ float cap_slope(const LossArgs &a, float x) {
-    if (!(FEAT & F_GENERAL) || !(a.cap > 0.0f))
+    if (!(FEAT & F_CAP))
         return 1.0f;
     const float r = cap_recip(a, x);
     return 4.0f * fmaf(-r, r, r);
@@ -947,11 +954,7 @@ __device__ __forceinline__ void write_listed(const LossArgs &a, const Row<TYPE> 
  * straight into LDS (a.stash per thread), and what is left is read twice. HELD = 0: no gradient is wanted, the row
  * is read as it comes by more wavefronts. */
 template <int TYPE, int OP, int FEAT> struct Held { /* what 128 registers have room for */
-    static constexpr int N = TYPE == GEIST_HIP_TYPE_F32        ? (FEAT & F_GENERAL ? 12 : 16)
-                             : FEAT == (F_GENERAL | F_ENTROPY) ? 4
-                             : FEAT & F_GENERAL                ? 8
-                             : OP == OP_DISTILL                ? 12
-                                                               : 16;
+    static constexpr int N = FEAT & (F_CAP | F_BITS) ? 12 : OP == OP_DISTILL ? 14 : 16;
 };
 constexpr int UH = 2;
 template <int TYPE, int OP, int FEAT, int THREADS, int HELD>
@@ -960,7 +963,7 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
     extern __shared__ __align__(16) char lds[];
     const int       row = blockIdx.x, tid = (int) threadIdx.x;
     const bool      lead = tid < 64; /* the wavefront that forms the row's scalars */
-    const bool      tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    const bool      tail = OP == OP_DISTILL && (FEAT & F_BITS) && a.tail;
     const Row<TYPE> r(a, row, 0, 1, 0);
     uint32_t       *map = nullptr;
     ListSums        ls  = {};
@@ -1004,7 +1007,7 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
                 some[i]     = raw[h + i];
                 if (v < r.nvec) {
                     keep[i] = bits.of(h + i);
-                    if ((FEAT & F_GENERAL) && map)
+                    if ((FEAT & F_BITS) && map)
                         keep[i] &= ~listed_bits<Elem<TYPE>::N>(map, v);
                     live |= 1u << i;
                 }
@@ -1019,7 +1022,7 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
         for (int h = 0; h < a.stash; ++h) {
             const int v = (HELD + h) * THREADS + tid;
             if (v < r.nvec) {
-                const u32x4    one[1]  = {stash[h * THREADS + tid]};
+                u32x4          one[1]  = {stash[h * THREADS + tid]};
                 const uint32_t keep[1] = {keep_bits<TYPE, FEAT>(a, r, map, v)};
                 acc_batch<TYPE, FEAT, 1>(a, acc, one, keep, 1u);
             }
@@ -1096,7 +1099,7 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
             return;
     }
     const Row<TYPE> r(a, row, chunk, a.chunks, a.chunk_vecs);
-    const bool      tail = OP == OP_DISTILL && (FEAT & F_GENERAL) && a.tail;
+    const bool      tail = OP == OP_DISTILL && (FEAT & F_BITS) && a.tail;
     const bool      lead = threadIdx.x < 64;
     Acc             acc;
     ListSums        ls = {};
@@ -1241,14 +1244,22 @@ void launch_loss(LossStage stage, int op, int feat, const LossArgs &a, size_t ld
 #define GS_CASE(OP, FEAT)                                                                       \
     if (op == OP && feat == (FEAT))                                                             \
         return launch_one<TYPE, OP, (FEAT)>(stage, a, lds, chunks, chunk_vecs, stream);
+    /* (soft-cap and mask together come with the entropy's sum, wanted or not) */
     GS_CASE(OP_TOKEN, 0)
     GS_CASE(OP_TOKEN, F_ENTROPY)
-    GS_CASE(OP_TOKEN, F_GENERAL)
-    GS_CASE(OP_TOKEN, F_GENERAL | F_ENTROPY)
+    GS_CASE(OP_TOKEN, F_CAP)
+    GS_CASE(OP_TOKEN, F_CAP | F_ENTROPY)
+    GS_CASE(OP_TOKEN, F_BITS)
+    GS_CASE(OP_TOKEN, F_BITS | F_ENTROPY)
+    GS_CASE(OP_TOKEN, F_CAP | F_BITS | F_ENTROPY)
     GS_CASE(OP_DISTILL, 0)
-    GS_CASE(OP_DISTILL, F_GENERAL)
+    GS_CASE(OP_DISTILL, F_CAP)
+    GS_CASE(OP_DISTILL, F_BITS)
+    GS_CASE(OP_DISTILL, F_CAP | F_BITS)
     GS_CASE(OP_PREFERENCE, 0)
-    GS_CASE(OP_PREFERENCE, F_GENERAL)
+    GS_CASE(OP_PREFERENCE, F_CAP)
+    GS_CASE(OP_PREFERENCE, F_BITS)
+    GS_CASE(OP_PREFERENCE, F_CAP | F_BITS)
 #undef GS_CASE
 }
 
