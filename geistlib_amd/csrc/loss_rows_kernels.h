@@ -169,17 +169,8 @@ template <int TYPE> struct Row {
         return *reinterpret_cast<const u32x4 *>(x + head + (long) v * N);
     }
     /* for what is not read again and cannot have come from the cache */
-    __device__ __forceinline__ u32x4 load(int v, bool streamed) const {
-        const u32x4 *p = reinterpret_cast<const u32x4 *>(x + head + (long) v * N);
-        u32x4        d;
-        if (streamed) {
-            asm volatile(""); /* (keeps the two loads from being made one, an ordinary one) */
-            d = __builtin_nontemporal_load(p);
-            asm volatile("");
-        } else {
-            d = *p;
-        }
-        return d;
+    __device__ __forceinline__ u32x4 load_streamed(int v) const {
+        return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + head + (long) v * N));
     }
     /* to the place of lane 0 in `wave`, each lane's 16 bytes behind it */
     __device__ __forceinline__ void load_to_lds(int v, u32x4 *wave, bool streamed) const {
@@ -452,23 +443,24 @@ __device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r,
         }
     }
 }
-/* the groups from v0 + `from` on, read as they come */
-template <int TYPE, int FEAT, int THREADS, int U>
+/* the groups from v0 + `from` on, read as they come. (Loads stand under no condition of a lane's: behind
+ * one, the compiler unpacks each group where it was loaded and so waits for every load by itself.) */
+template <int TYPE, int FEAT, int THREADS, int U, bool STREAMED>
 __device__ __forceinline__ void sum_groups(const LossArgs &a, const Row<TYPE> &r, const uint32_t *map,
-                                           int from, bool streamed, Acc &c) {
+                                           int from, Acc &c) {
     bool start = from == 0;
     for (int v = r.v0 + from + (int) threadIdx.x; v < r.v1; v += U * THREADS) {
         u32x4    raw[U];
         uint32_t keep[U], live = 0;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            keep[j] = 0;
-            if (v + j * THREADS < r.v1) {
-                raw[j]  = r.load(v + j * THREADS, streamed);
-                keep[j] = keep_bits<TYPE, FEAT>(a, r, map, v + j * THREADS);
-                live |= 1u << j;
-            }
+            const int w = min(v + j * THREADS, r.v1 - 1);
+            raw[j]      = STREAMED ? r.load_streamed(w) : r.load(w);
+            live |= v + j * THREADS < r.v1 ? 1u << j : 0u;
         }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            keep[j] = keep_bits<TYPE, FEAT>(a, r, map, min(v + j * THREADS, r.v1 - 1));
         if (start)
             acc_move(c, group_top<TYPE, FEAT>(a, raw[0], keep[0]), a.k);
         start = false;
@@ -659,10 +651,10 @@ __device__ __forceinline__ void write_groups(const LossArgs &a, const Row<TYPE> 
         uint32_t keep[U];
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            if (v + i * THREADS < r.v1) {
-                raw[i]  = r.load(v + i * THREADS);
-                keep[i] = keep_bits<TYPE, FEAT>(a, r, nullptr, v + i * THREADS);
-            }
+            raw[i] = r.load(min(v + i * THREADS, r.v1 - 1));
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            keep[i] = keep_bits<TYPE, FEAT>(a, r, nullptr, min(v + i * THREADS, r.v1 - 1));
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (v + i * THREADS < r.v1)
@@ -703,19 +695,17 @@ template <int TYPE> struct Token {
     uint32_t                 may;
     /* softcap(x) k; -inf where the token is forbidden */
     template <int FEAT> __device__ __forceinline__ double w(const LossArgs &a) const {
-        return !(may & 1u) ? -INFINITY : value64<TYPE, FEAT>(a, Elem<TYPE>::one(x));
+        return !((may >> (max(id, 0) & 31)) & 1u) ? -INFINITY : value64<TYPE, FEAT>(a, Elem<TYPE>::one(x));
     }
 };
 /* (only asked for here: what was asked for before need not have arrived) */
 template <int TYPE> __device__ __forceinline__ Token<TYPE> load_token(const LossArgs &a, const Row<TYPE> &r, int row) {
-    Token<TYPE> t = {};
+    Token<TYPE> t;
     t.id          = a.tokens[row];
-    if (t.id < 0 || t.id >= r.n) {
-        t.id = -1;
-    } else {
-        t.x   = r.x[t.id];
-        t.may = r.allowed ? r.allowed[t.id >> 5] >> (t.id & 31) : 1u;
-    }
+    t.id          = t.id < 0 || t.id >= r.n ? -1 : t.id;
+    const int at  = max(t.id, 0);
+    t.x           = r.x[at];
+    t.may         = r.allowed ? r.allowed[at >> 5] : ~0u;
     return t;
 }
 /* Policy loss of a row from its sums; `lead`: this thread writes the row's outputs. */
@@ -977,10 +967,18 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
     Acc   acc;
     u32x4 raw[HELD ? HELD : 1];
     if constexpr (HELD > 0) {
+        if (r.nvec > 0) {
+            if (a.streamed) {
 #pragma unroll
-        for (int h = 0; h < HELD; ++h)
-            if (h * THREADS + tid < r.nvec)
-                raw[h] = r.load(h * THREADS + tid, a.streamed);
+                for (int h = 0; h < HELD; ++h)
+                    raw[h] = r.load_streamed(min(h * THREADS + tid, r.nvec - 1));
+                asm volatile(""); /* (keeps the two kinds of loads from being made one) */
+            } else {
+#pragma unroll
+                for (int h = 0; h < HELD; ++h)
+                    raw[h] = r.load(min(h * THREADS + tid, r.nvec - 1));
+            }
+        }
     }
     /* [stash][THREADS] groups, each the own thread's */
     u32x4 *const stash = reinterpret_cast<u32x4 *>(lds + a.stash_at);
@@ -1027,9 +1025,12 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
                 acc_batch<TYPE, FEAT, 1>(a, acc, one, keep, 1u);
             }
         }
-        sum_groups<TYPE, FEAT, THREADS, UH>(a, r, map, (HELD + a.stash) * THREADS, false, acc);
+        sum_groups<TYPE, FEAT, THREADS, UH, false>(a, r, map, (HELD + a.stash) * THREADS, acc);
     } else {
-        sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, a.streamed, acc);
+        if (a.streamed)
+            sum_groups<TYPE, FEAT, THREADS, 4, true>(a, r, map, 0, acc);
+        else
+            sum_groups<TYPE, FEAT, THREADS, 4, false>(a, r, map, 0, acc);
     }
     acc_loose<TYPE, FEAT>(a, r, map, acc);
     Sums j = join_threads<FEAT, THREADS>(acc, sh);
@@ -1112,10 +1113,13 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
             ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), map, nullptr);
         if (tail)
             lds_barrier();
-    } else if (chunk == 0) {
+    } else {
         t = load_token<TYPE>(a, r, row);
     }
-    sum_groups<TYPE, FEAT, THREADS, 4>(a, r, map, 0, row < a.streamed_rows, acc);
+    if (row < a.streamed_rows)
+        sum_groups<TYPE, FEAT, THREADS, 4, true>(a, r, map, 0, acc);
+    else
+        sum_groups<TYPE, FEAT, THREADS, 4, false>(a, r, map, 0, acc);
     acc_loose<TYPE, FEAT>(a, r, map, acc);
     Sums j = join_threads<FEAT, THREADS>(acc, sh);
     if (needs_care(j))
