@@ -29,21 +29,33 @@ struct LossPart {
 };
 
 struct LossPlan {
-    int chunks;     /* workgroups per row of the pass that sums; 1 with a gradient: one launch */
-    int chunk_vecs; /* groups of 16 bytes each of them takes */
+    int chunks;     /* parts a row is cut into; 1 and not a preference loss: one launch does the rows */
+    int chunk_vecs; /* groups of 16 bytes each of them has */
 };
 
 constexpr size_t LOSS_MAP_MOST  = (size_t) 1 << 18; /* logits per workgroup its bit map has room for (32 KB) */
+constexpr int    LOSS_WIDE_ROWS = 256;              /* up to a row per compute unit: wide workgroups */
 constexpr size_t LOSS_GRID_MOST = 0x3fffff;         /* workgroups per launch (of up to 1024 threads) */
 
-/* How a call over rows x n logits of `elem` bytes is cut. */
-inline LossPlan loss_plan(size_t rows, size_t n, size_t elem) {
-    const size_t vecs = n * elem / 16 + 1;
+enum LossUse { LOSS_ALONE, LOSS_AND_GRADIENT, LOSS_PREFERENCE };
+
+/* How a call over rows x n logits of `elem` bytes is cut. One launch with a workgroup per row reads every
+ * logit once; two launches over parts of the rows read them twice and pay a launch more, but spread a few
+ * long rows over the device. Measured, one launch against two (us):
+ *   with a gradient  1 x 262 KB 15.3 / 8.4, 32 x 257 KB about equal, 16 x 524 KB 30.1 / 12.4,
+ *                    64 x 513 KB 25.4 / 20.2 (with a list 26.3 / 32.4), 128 x 513 KB 35.5 / 43.1
+ *   loss alone       1 x 257 KB 8.1 / 7.4, 64 x 257 KB 9.2 / 9.6, 16 x 524 KB 13.5 / 8.2, 128 x 524 KB 17.0 / 17.3
+ * The preference loss has its sums and its gradient in two launches whatever the sizes; its parts of 64 KB
+ * cost a large batch nothing (1760 x 257 KB: 264 us whole, 267 cut) and spread a small one
+ * (16 x 257 KB 40.2 / 20.1). */
+inline LossPlan loss_plan(size_t rows, size_t n, size_t elem, LossUse use) {
+    const size_t vecs = n * elem / 16 + 1, row_bytes = n * elem;
     LossPlan     p    = {1, (int) vecs};
-    /* too few rows to fill the device with one workgroup each, or a row that is too long for one */
-    size_t chunks = 1;
-    if (rows < 512)
-        chunks = std::min<size_t>((1024 + rows - 1) / rows, (vecs + 1023) / 1024);
+    size_t       chunks = 1;
+    if (use == LOSS_PREFERENCE)
+        chunks = rows < 64 ? (vecs + 2047) / 2048 : (vecs + 4095) / 4096;
+    else if (row_bytes > 200000 && rows <= (use == LOSS_AND_GRADIENT && row_bytes > 400000 ? 64 : 32))
+        chunks = std::min((vecs + 1023) / 1024, 2048 / rows);
     chunks = std::max(chunks, (n + LOSS_MAP_MOST - 1) / LOSS_MAP_MOST);
     if (chunks > 1) {
         p.chunk_vecs = (int) ((vecs + chunks - 1) / chunks);
@@ -52,11 +64,16 @@ inline LossPlan loss_plan(size_t rows, size_t n, size_t elem) {
     return p;
 }
 
+inline size_t loss_chunks_most(size_t rows, size_t n, size_t elem) {
+    int most = 1;
+    for (LossUse use : {LOSS_ALONE, LOSS_AND_GRADIENT, LOSS_PREFERENCE})
+        most = std::max(most, loss_plan(rows, n, elem, use).chunks);
+    return (size_t) most;
+}
 inline size_t loss_workspace_bytes(size_t rows, size_t n_vocab) {
     if (rows == 0 || n_vocab == 0 || rows > LOSS_GRID_MOST || n_vocab > 0x7fffff00u)
         return 0;
-    const size_t chunks = (size_t) std::max(loss_plan(rows, n_vocab, 2).chunks,
-                                            loss_plan(rows, n_vocab, 4).chunks);
+    const size_t chunks = std::max(loss_chunks_most(rows, n_vocab, 2), loss_chunks_most(rows, n_vocab, 4));
     return (rows * (chunks * sizeof(LossPart) + sizeof(float)) + 15) / 16 * 16;
 }
 
@@ -85,7 +102,7 @@ inline int check_loss_rows(const geist_hip_loss_rows *r, const void *ws, size_t 
         return refuse(why, GEIST_HIP_E_INVALID_ARG, "n_vocab too large");
     const size_t elem = r->type == GEIST_HIP_TYPE_F32 ? 4 : 2;
     if (r->rows > LOSS_GRID_MOST ||
-        (size_t) loss_plan(r->rows, r->n_vocab, elem).chunks * r->rows > LOSS_GRID_MOST)
+        loss_chunks_most(r->rows, r->n_vocab, elem) * r->rows > LOSS_GRID_MOST)
         return refuse(why, GEIST_HIP_E_UNSUPPORTED, "%zu rows of %zu logits in one call", r->rows,
                       r->n_vocab);
     if (r->ld < r->n_vocab || r->ld > ((size_t) 1 << 58) / r->rows)

@@ -117,9 +117,12 @@ constexpr size_t CACHE_BYTES = (size_t) 224 << 20, KEPT_BYTES = (size_t) 160 << 
 
 size_t elem_bytes(int type) { return type == GEIST_HIP_TYPE_F32 ? 4 : 2; }
 
-LossArgs args_of(const geist_hip_loss_rows &r, void *ws) {
+LossArgs args_of(const geist_hip_loss_rows &r, void *ws, bool preference = false) {
     LossArgs       a    = {};
-    const LossPlan plan = loss_plan(r.rows, r.n_vocab, elem_bytes(r.type));
+    const LossPlan plan = loss_plan(r.rows, r.n_vocab, elem_bytes(r.type),
+                                          preference ? LOSS_PREFERENCE
+                                          : r.d_grad ? LOSS_AND_GRADIENT
+                                                     : LOSS_ALONE);
     a.x          = r.d_logits;
     a.g          = r.d_grad;
     a.ld         = (long) r.ld;
@@ -214,7 +217,7 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
 
 void launch_preference(const geist_hip_loss_rows &r, const geist_hip_preference &p, float *loss,
                        float *ratios, float *logprob, void *ws, hipStream_t stream) {
-    LossArgs a  = args_of(r, ws);
+    LossArgs a  = args_of(r, ws, true);
     a.coef      = r.d_grad ? reinterpret_cast<float *>(a.part + r.rows * (size_t) a.chunks) : nullptr;
     a.tokens    = p.d_tokens;
     a.ref_lp    = p.d_ref;

@@ -1208,7 +1208,9 @@ void launch_one(LossStage stage, const LossArgs &a, size_t lds, int chunks, int 
         if constexpr (OP != OP_PREFERENCE) {
             constexpr int H    = Held<TYPE, OP, FEAT>::N;
             const int     vecs = a.n / Elem<TYPE>::N, need = vecs / H;
-            if (!a.g) {
+            if (!a.g && a.rows <= LOSS_WIDE_ROWS && vecs >= 4096) {
+                k_loss_row<TYPE, OP, FEAT, 1024, 0><<<dim3(a.rows), 1024, lds, stream>>>(a);
+            } else if (!a.g) {
                 k_loss_row<TYPE, OP, FEAT, 256, 0><<<dim3(a.rows), 256, lds, stream>>>(a);
             } else if (need <= 128) {
                 k_loss_row<TYPE, OP, FEAT, 128, H><<<dim3(a.rows), 128, lds, stream>>>(a);

@@ -141,8 +141,9 @@ int main() {
     for (size_t rows : {(size_t) 1, (size_t) 3, (size_t) 64, (size_t) 511, (size_t) 512, (size_t) 5000})
         for (size_t n : {(size_t) 1, (size_t) 7, (size_t) 4096, (size_t) 8191, (size_t) 50257,
                          (size_t) 262144, (size_t) 262145, (size_t) 1 << 24, (size_t) 0x7fffff00u})
-            for (size_t elem : {(size_t) 2, (size_t) 4}) {
-                const LossPlan p    = loss_plan(rows, n, elem);
+            for (size_t elem : {(size_t) 2, (size_t) 4})
+            for (LossUse use : {LOSS_ALONE, LOSS_AND_GRADIENT, LOSS_PREFERENCE}) {
+                const LossPlan p    = loss_plan(rows, n, elem, use);
                 const size_t   vecs = n * elem / 16, held = (size_t) p.chunks * p.chunk_vecs;
                 if (p.chunks < 1 || p.chunk_vecs < 1 || held < vecs ||
                     (size_t) (p.chunks - 1) * p.chunk_vecs > vecs ||

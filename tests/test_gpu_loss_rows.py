@@ -605,3 +605,135 @@ def test_sampled_scored_and_trained_on(hs, oracle):
     sampler.sync()
     assert float(l0.abs().max()) < 2e-5 and float(grad.abs().max()) < 2e-5
     sampler.close()
+
+
+# few long rows, cut into parts; and long rows of larger batches, of which a workgroup holds a part in
+# registers, a part in LDS and reads the rest twice
+LONG = [(2, 60001, "f32", 1, 3), (3, 130003, "bf16", 3, 0), (1, 300000, "f16", 0, 0), (40, 110001, "f32", 0, 0)]
+HELD_ROWS = [(66, 60000, "f32", 0, 0), (70, 262144, "f32", 0, 0), (34, 131075, "bf16", 1, 2), (65, 262143, "f16", 0, 1),
+        (40, 250001, "bf16", 0, 0)]
+
+
+@pytest.mark.parametrize("temperature,cap,masked", OPTIONS)
+@pytest.mark.parametrize("rows,n,dtype,lead,pad", LONG + HELD_ROWS)
+def test_long_rows(hs, rows, n, dtype, lead, pad, temperature, cap, masked):
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n)
+    base = logits(g, 3, n)
+    x = base[np.arange(rows) % 3]
+    allowed = None
+    if masked:
+        allowed = mask_of(g, 3, n, True)[np.arange(rows) % 3]
+    look = sorted({0, min(1, rows - 1), min(2, rows - 1), rows - 1})
+    b = Batch(x, dtype, lead, pad, allowed=allowed, temperature=temperature, cap=cap)
+    weight = g.uniform(0.1, 2, rows).astype(np.float32)
+    d_w = dev(weight)
+    ids, values = distill_inputs(g, rows, n, 50)
+    d_ids, d_val = dev(ids), dev(values)
+    loss = out(rows)
+    for tail in (False, True):
+        hs.distill(b.view, HipSampler.teacher(d_ids, d_val, weight=d_w, tail=tail), loss, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in look:
+            want, gr, tol, g_tol = ref.distill(b.x[r], dtype, ids[r], values[r], tail, temperature, cap,
+                                               None if allowed is None else allowed[r], float(weight[r]))
+            near(loss[r].item(), want, tol, f"tail {tail}: loss of row {r}")
+            near(grads[r], gr, g_tol, f"tail {tail}: gradient of row {r}")
+        alone = out(rows)
+        view = HipSampler.loss_rows(b.logits, allowed=b.d_allowed, temperature=temperature, softcap=cap)
+        hs.distill(view, HipSampler.teacher(d_ids, d_val, weight=d_w, tail=tail), alone, b.ws)
+        hs.sync()
+        near(alone.cpu(), loss.cpu(), loss.abs().cpu() * 3e-6 + 1e-7, "loss alone")
+    tokens = np.argmax(b.x, 1).astype(np.int32)
+    tokens[1::3] = n // 2
+    advantage = g.standard_normal(rows).astype(np.float32)
+    d_tok, d_adv = dev(tokens), dev(advantage)
+    lp, ent = out(rows), out(rows)
+    p = HipSampler.policy(d_tok, d_adv, weight=d_w, entropy_coef=0.01)
+    hs.policy_loss(b.view, p, loss, lp, ent, b.ws)
+    hs.sync()
+    grads = b.grads()
+    for r in look:
+        want = ref.policy(b.x[r], dtype, int(tokens[r]), float(advantage[r]), None, None, float(weight[r]),
+                          ent=float(np.float32(0.01)), temperature=temperature, cap=cap,
+                          allowed=None if allowed is None else allowed[r])
+        for name, got in (("loss", loss), ("logprob", lp), ("entropy", ent)):
+            near(got[r].item(), want[name], want[name + "_tol"] + abs(want[name]) * 2.0 ** -23
+                 if np.isfinite(want[name]) else 0.0, f"{name} of row {r}")
+        near(grads[r], want["grad"], want["grad_tol"], f"gradient of row {r}")
+    lp2, ent2 = out(rows), out(rows)
+    view = HipSampler.loss_rows(b.logits, allowed=b.d_allowed, temperature=temperature, softcap=cap)
+    hs.policy_loss(view, p, loss, lp2, ent2, b.ws)
+    hs.sync()
+    near(lp2.cpu(), lp.cpu(), lp.abs().cpu() * 3e-6 + 1e-6, "logprob alone")
+    near(ent2.cpu(), ent.cpu(), ent.abs().cpu() * 3e-6 + 1e-6, "entropy alone")
+    # in the place of the logits: the same bits
+    want = b.grad.clone()
+    c = Batch(x, dtype, lead, pad, grad="in place", allowed=allowed, temperature=temperature, cap=cap)
+    hs.policy_loss(c.view, p, loss, lp, ent, c.ws)
+    hs.sync()
+    assert torch.equal(c.grad, want)
+
+
+def test_long_rows_of_special_values(hs):
+    """Parts of rows, and what LDS holds of a row, without anything that counts: all masked, of the lowest
+    value, NaN behind the mask."""
+    from geistlib_amd import HipSampler
+    for rows in (3, 70):
+        n = 150000
+        x = np.zeros((rows, n))
+        x[0, 100:] = -np.finfo(np.float32).max     # what counts lies in the first part
+        x[1, :-5] = -np.inf                        # ... in the last one
+        x[2, 70000:] = np.nan                      # behind the mask
+        allowed = np.ones((rows, n), bool)
+        allowed[2, 60000:] = False
+        b = Batch(x, "f32", allowed=allowed)
+        d_tok, d_adv = dev(np.full(rows, 3, np.int32)), dev(np.ones(rows, np.float32))
+        loss, lp, ent = out(rows), out(rows), out(rows)
+        hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, entropy_coef=0.1), loss, lp, ent, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in range(3):
+            want = ref.policy(b.x[r], "f32", 3, 1.0, None, None, ent=float(np.float32(0.1)), allowed=allowed[r])
+            near(ent[r].item(), want["entropy"], want["entropy_tol"] + want["entropy"] * 2.0 ** -23, f"entropy {r}")
+            near(lp[r].item(), want["logprob"], want["logprob_tol"] + 1e-6, f"logprob {r}")
+            near(grads[r], want["grad"], want["grad_tol"], f"gradient {r}")
+
+
+def test_a_batch_beyond_the_cache(hs):
+    """Non-temporal reads and writes, the preference loss's second pass from the last row back: the same
+    bits as smaller batches of the same rows give."""
+    from geistlib_amd import HipSampler
+    rows, n = 1300, 131072
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn((rows, n), generator=gen, device="cuda") * 2).to(torch.bfloat16)
+    g = np.random.default_rng(5)
+    tokens = g.integers(0, n, rows).astype(np.int32)
+    d_tok, d_adv = dev(tokens), dev(g.standard_normal(rows).astype(np.float32))
+    d_start = dev(np.array([0, 300, 650, 1000, 1300], np.int32))
+    ws = torch.empty(HipSampler.loss_workspace_bytes(rows, n), dtype=torch.uint8, device="cuda")
+    grad = torch.empty_like(x)
+    loss, lp = out(rows), out(rows)
+    hs.policy_loss(HipSampler.loss_rows(x, grad=grad), HipSampler.policy(d_tok, d_adv), loss, lp, None, ws)
+    part = torch.empty((100, n), dtype=torch.bfloat16, device="cuda")
+    loss2, lp2 = out(100), out(100)
+    for r in (0, 600, 1200):
+        hs.policy_loss(HipSampler.loss_rows(x[r:r + 100], grad=part),
+                       HipSampler.policy(d_tok[r:r + 100], d_adv[r:r + 100]), loss2, lp2, None, ws)
+        hs.sync()
+        assert torch.equal(part, grad[r:r + 100]) and torch.equal(lp2, lp[r:r + 100])
+        assert torch.equal(loss2, loss[r:r + 100])
+    p_loss, ratios = out(2), out(4)
+    hs.preference_loss(HipSampler.loss_rows(x, grad=grad), HipSampler.preference(d_tok, d_start), p_loss,
+                       ratios, lp, ws)
+    hs.sync()
+    for r in (0, 299, 300, 649, 1299):
+        want = ref.policy(x[r].float().cpu().numpy(), "bf16", int(tokens[r]), 1.0, None, None)
+        near(lp[r].item(), want["logprob"], want["logprob_tol"] + 1e-6, f"logprob {r}")
+    half = torch.empty((650, n), dtype=torch.bfloat16, device="cuda")
+    d_s2 = dev(np.array([0, 350, 650], np.int32))
+    hs.preference_loss(HipSampler.loss_rows(x[650:], grad=half), HipSampler.preference(d_tok[650:], d_s2),
+                       p_loss[:1].clone(), ratios[:2].clone(), None, ws)
+    hs.sync()
+    assert torch.equal(half, grad[650:])
