@@ -283,16 +283,13 @@ __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_
     if (FEAT & F_BITS) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t on = bit_mask(keep, i);
-            e[i]              = __uint_as_float(__float_as_uint(e[i]) & on);
-            if (FEAT & F_ENTROPY)
-                u[i] = __uint_as_float(__float_as_uint(u[i]) & on);
+            e[i] = __uint_as_float(__float_as_uint(e[i]) & bit_mask(keep, i));
         }
     }
-    if (FEAT & F_ENTROPY) { /* 0 * -inf is no term of an entropy */
+    if (FEAT & F_ENTROPY) { /* finite, whatever stands behind a mask: 0 * -inf is no term of an entropy */
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            u[i] = fmaxf(u[i], -1e30f);
+            u[i] = FEAT & F_BITS ? __builtin_amdgcn_fmed3f(u[i], -1e30f, 1e30f) : fmaxf(u[i], -1e30f);
     }
 }
 /* Listed tokens of the workgroup's part of the row as bits (tail only): group v's start at bit
@@ -620,7 +617,7 @@ __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32
         g[i] = e[i] * ((FEAT & F_ENTROPY) ? fmaf(c.b, u[i], c.a) : c.a);
         if (FEAT & F_CAP) /* 1 - tanh^2 = 4 (r - r^2) */
             g[i] *= 4.0f * fmaf(-r[i], r[i], r[i]);
-        if (FEAT & F_BITS) /* (a forbidden NaN has no slope either) */
+        if ((FEAT & F_BITS) && (FEAT & F_CAP)) /* (a forbidden NaN has no slope either) */
             g[i] = __uint_as_float(__float_as_uint(g[i]) & bit_mask(keep, i));
     }
     return Elem<TYPE>::pack(g);
@@ -1202,36 +1199,50 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
 constexpr int LDS_MOST = 158 * 1024; /* of 160 KB; the rest is what a kernel declares itself */
 static_assert(sizeof(Shared) <= 2048, "beside the dynamic part");
 
+/* groups per thread that go to LDS, of which a workgroup may use its share of the compute unit's */
+template <int HELD> int stash_of(int threads, int vecs, size_t lds) {
+    const int room = LDS_MOST * threads / 1024 - (int) ((lds + 15) / 16 * 16);
+    return std::max(0, std::min(room / (threads * 16), (vecs + threads - 1) / threads - HELD));
+}
+template <int TYPE, int OP, int FEAT, int THREADS, int HELD>
+void launch_held(LossArgs a, int vecs, size_t lds, hipStream_t stream) {
+    a.stash          = stash_of<HELD>(THREADS, vecs, lds);
+    a.stash_at       = (int) ((lds + 15) / 16 * 16);
+    const size_t all = (size_t) a.stash_at + (size_t) a.stash * THREADS * 16;
+    auto        *k   = k_loss_row<TYPE, OP, FEAT, THREADS, HELD>;
+    /* (more than a launch gets unasked; where it is refused so is the launch, which the caller sees) */
+    if (all > 64 * 1024)
+        (void) hipFuncSetAttribute(reinterpret_cast<const void *>(k),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MOST);
+    k<<<dim3(a.rows), THREADS, all, stream>>>(a);
+}
+
 template <int TYPE, int OP, int FEAT>
 void launch_one(LossStage stage, const LossArgs &a, size_t lds, int chunks, int chunk_vecs, hipStream_t stream) {
     if (stage == STAGE_ROW) {
         if constexpr (OP != OP_PREFERENCE) {
-            constexpr int H    = Held<TYPE, OP, FEAT>::N;
-            const int     vecs = a.n / Elem<TYPE>::N, need = vecs / H;
+            const int vecs = a.n / Elem<TYPE>::N;
             if (!a.g && a.rows <= LOSS_WIDE_ROWS && vecs >= 4096) {
                 k_loss_row<TYPE, OP, FEAT, 1024, 0><<<dim3(a.rows), 1024, lds, stream>>>(a);
             } else if (!a.g) {
                 k_loss_row<TYPE, OP, FEAT, 256, 0><<<dim3(a.rows), 256, lds, stream>>>(a);
-            } else if (need <= 128) {
-                k_loss_row<TYPE, OP, FEAT, 128, H><<<dim3(a.rows), 128, lds, stream>>>(a);
-            } else if (need <= 256) {
-                k_loss_row<TYPE, OP, FEAT, 256, H><<<dim3(a.rows), 256, lds, stream>>>(a);
-            } else if (need <= 512) {
-                k_loss_row<TYPE, OP, FEAT, 512, H><<<dim3(a.rows), 512, lds, stream>>>(a);
             } else {
-                /* one workgroup to a compute unit: all of its LDS is free for the row */
-                LossArgs  b    = a;
-                const int most = (LDS_MOST - (int) ((lds + 15) / 16 * 16)) / (1024 * 16);
-                b.stash        = std::max(0, std::min(most, vecs / 1024 + 1 - H));
-                b.stash_at     = (int) ((lds + 15) / 16 * 16);
-                const size_t all = (size_t) b.stash_at + (size_t) b.stash * 1024 * 16;
-                auto        *k   = k_loss_row<TYPE, OP, FEAT, 1024, H>;
-                /* (more than a launch gets unasked; where it is refused so is the launch, which the caller
-                 * sees) */
-                if (all > 64 * 1024)
-                    (void) hipFuncSetAttribute(reinterpret_cast<const void *>(k),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MOST);
-                k<<<dim3(a.rows), 1024, all, stream>>>(b);
+                constexpr int H = Held<TYPE, OP, FEAT>::N;
+                /* the smallest workgroup that holds the row, so that several share a compute unit and one
+                 * loads while another computes; 512 threads also where they hold three quarters of it
+                 * (4096 x 128256 bf16, of which they hold 80 %: 388 us, 1024 threads 401; 512 x 151936
+                 * f32, 24 %: 159, 1024 threads 144). With no more rows than compute units none is shared:
+                 * as many threads as there are. */
+                auto held = [&](int threads) { return (H + stash_of<H>(threads, vecs, lds)) * threads; };
+                const bool few = a.rows <= LOSS_WIDE_ROWS && vecs >= 4096;
+                if (!few && held(128) >= vecs)
+                    launch_held<TYPE, OP, FEAT, 128, H>(a, vecs, lds, stream);
+                else if (!few && held(256) >= vecs)
+                    launch_held<TYPE, OP, FEAT, 256, H>(a, vecs, lds, stream);
+                else if (!few && held(512) >= vecs / 4 * 3)
+                    launch_held<TYPE, OP, FEAT, 512, H>(a, vecs, lds, stream);
+                else
+                    launch_held<TYPE, OP, FEAT, 1024, H>(a, vecs, lds, stream);
             }
         }
     } else if (stage == STAGE_SUMS) {
