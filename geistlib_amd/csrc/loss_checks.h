@@ -28,6 +28,12 @@ struct LossPart {
     int    careful; /* the sums were made against a value m outside the range of plain references */
 };
 
+/* What the gradient of a row of the preference loss takes: 2^(w - ref) a, - q at the token. */
+struct LossRowGrad {
+    float a, ref, q;
+    int   kind; /* 0: zeros; 1; 2: careful, the exponent is (y - ref) k */
+};
+
 struct LossPlan {
     int chunks;     /* parts a row is cut into; 1 and not a preference loss: one launch does the rows */
     int chunk_vecs; /* groups of 16 bytes each of them has */
@@ -74,7 +80,7 @@ inline size_t loss_workspace_bytes(size_t rows, size_t n_vocab) {
     if (rows == 0 || n_vocab == 0 || rows > LOSS_GRID_MOST || n_vocab > 0x7fffff00u)
         return 0;
     const size_t chunks = std::max(loss_chunks_most(rows, n_vocab, 2), loss_chunks_most(rows, n_vocab, 4));
-    return (rows * (chunks * sizeof(LossPart) + sizeof(float)) + 15) / 16 * 16;
+    return (rows * (chunks * sizeof(LossPart) + sizeof(LossRowGrad)) + 15) / 16 * 16;
 }
 
 /* Each check returns a status code and leaves the reason of a refusal in `why`. */

@@ -52,7 +52,7 @@ struct LossArgs {
     /* preference */
     const int32_t  *seq_start;
     int             n_pairs;
-    float          *coef; /* [rows] d loss / d logprob */
+    LossRowGrad    *row_grad; /* [rows] */
     float          *ratios;
     int             kind, length_normalised;
     float           beta, margin, smoothing;

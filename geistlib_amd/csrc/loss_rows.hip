@@ -38,22 +38,44 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
         const bool      used = id >= 0 && id < a.n;
         double          lp   = 0.0;
         if (used) {
-            double c = p[0].c, s = 0.0;
-            for (int i = 1; i < a.chunks; ++i)
-                c = fmax(c, p[i].c);
+            /* the parts joined, as join_parts does it */
+            double top = p[0].c;
+            bool   careful = p[0].careful;
+            for (int i = 1; i < a.chunks; ++i) {
+                top = fmax(top, p[i].c);
+                careful |= p[i].careful != 0;
+            }
+            float m = -FLT_MAX;
+            bool  plain = false;
             for (int i = 0; i < a.chunks; ++i)
-                s += p[i].s * (double) __builtin_amdgcn_exp2f((float) fmax(p[i].c - c, -1e30));
-            lp = s == 0.0 ? -INFINITY : (p[0].a - c - log2(s)) * LN2;
+                if (p[i].c == top) {
+                    plain |= p[i].careful == 0;
+                    if (p[i].careful)
+                        m = fmaxf(m, p[i].m);
+                }
+            float        at  = careful ? (plain ? (float) (top / (double) a.k) : m) : (float) top;
+            const double ref = careful ? (double) at * (double) a.k : (double) at;
+            double       s   = 0.0;
+            for (int i = 0; i < a.chunks; ++i)
+                s += p[i].s * (double) __builtin_amdgcn_exp2f((float) fmax(p[i].c - ref, -1e30));
+            const double l2s = log2(s);
+            lp               = s == 0.0 ? -INFINITY : (p[0].a - ref - l2s) * LN2;
             if (lp != -INFINITY) {
                 const int side = row < edge[1] ? 0 : 1;
                 v[side] += a.ref_lp ? lp - (double) a.ref_lp[row] : lp;
                 v[2 + side] += 1.0;
             }
+            if (a.row_grad) {
+                /* against ref + log2(s) where that is a plain reference: the sum is then near 1 */
+                if (!careful) {
+                    at = (float) (ref + l2s);
+                    s *= exp2(ref - (double) at);
+                }
+                a.row_grad[row] = {(float) (1.0 / s), at, 0.0f, lp == -INFINITY ? 0 : careful ? 2 : 1};
+            }
         }
         if (a.logprob)
             a.logprob[row] = (float) lp;
-        if (a.coef) /* marks the rows that count */
-            a.coef[row] = used && lp != -INFINITY ? 1.0f : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -102,10 +124,19 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
             a.ratios[2 * pair + 1] = (float) ratio[1];
         }
     }
-    if (a.coef) {
-        const float c0 = (float) (d * w * share[0]), c1 = (float) (-d * w * share[1]);
-        for (int row = edge[0] + (int) threadIdx.x; row < edge[2]; row += PAIR_THREADS)
-            a.coef[row] = a.coef[row] == 0.0f ? 0.0f : row < edge[1] ? c0 : c1;
+    if (a.row_grad) {
+        const double c0 = d * w * share[0] * a.inv_t, c1 = -d * w * share[1] * a.inv_t;
+        for (int row = edge[0] + (int) threadIdx.x; row < edge[2]; row += PAIR_THREADS) {
+            LossRowGrad g = a.row_grad[row];
+            if (g.kind == 0)
+                continue;
+            const double dlp = row < edge[1] ? c0 : c1;
+            g.a              = (float) (-dlp * (double) g.a);
+            g.q              = (float) -dlp;
+            if (dlp == 0.0)
+                g.kind = 0;
+            a.row_grad[row] = g;
+        }
     }
 }
 
@@ -114,6 +145,8 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
  * (729 MB of sums 138 -> 121 us); where a second pass follows, all but the last of them, which that pass
  * reads first. */
 constexpr size_t CACHE_BYTES = (size_t) 224 << 20, KEPT_BYTES = (size_t) 160 << 20;
+
+constexpr size_t GRAD_VECS = 1024; /* groups of 16 bytes per workgroup of the second launch */
 
 size_t elem_bytes(int type) { return type == GEIST_HIP_TYPE_F32 ? 4 : 2; }
 
@@ -153,7 +186,15 @@ void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArg
     entropy        = entropy || (op == OP_TOKEN && rows == (F_CAP | F_BITS));
     const int feat = rows | (entropy ? F_ENTROPY : 0);
     /* without a gradient the second launch only writes the rows' outputs */
-    const int c = a.g ? a.chunks : 1, v = a.g ? a.chunk_vecs : INT32_MAX / 64;
+    int c = 1, v = INT32_MAX / 64;
+    if (stage == STAGE_GRAD && a.g) {
+        const size_t vecs = (size_t) a.n * elem_bytes(type) / 16 + 1;
+        size_t       per  = GRAD_VECS;
+        while ((size_t) a.rows * ((vecs + per - 1) / per) > LOSS_GRID_MOST)
+            per *= 2;
+        c = (int) ((vecs + per - 1) / per);
+        v = (int) per;
+    }
     if (type == GEIST_HIP_TYPE_F32)
         launch_loss<GEIST_HIP_TYPE_F32>(stage, op, feat, a, lds, c, v, stream);
     else if (type == GEIST_HIP_TYPE_F16)
@@ -218,7 +259,7 @@ void launch_distill(const geist_hip_loss_rows &r, const geist_hip_teacher &t, fl
 void launch_preference(const geist_hip_loss_rows &r, const geist_hip_preference &p, float *loss,
                        float *ratios, float *logprob, void *ws, hipStream_t stream) {
     LossArgs a  = args_of(r, ws, true);
-    a.coef      = r.d_grad ? reinterpret_cast<float *>(a.part + r.rows * (size_t) a.chunks) : nullptr;
+    a.row_grad  = r.d_grad ? reinterpret_cast<LossRowGrad *>(a.part + r.rows * (size_t) a.chunks) : nullptr;
     a.tokens    = p.d_tokens;
     a.ref_lp    = p.d_ref;
     a.seq_start = p.d_seq_start;

@@ -1121,15 +1121,17 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
     Sums j = join_threads<FEAT, THREADS>(acc, sh);
     if (needs_care(j))
         j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
-    if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.coef)
-        a.coef[row] = 0.0f;
+    if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.row_grad)
+        a.row_grad[row] = {0.0f, 0.0f, 0.0f, 0}; /* (of no pair yet) */
     if (threadIdx.x == 0)
         a.part[(long) row * a.chunks + chunk] = {
             j.s, j.t, j.ref(a.k), OP == OP_DISTILL ? ls.q_u : t.template w<FEAT>(a), ls.listed, ls.top, j.m, j.careful};
 }
 
 /* The gradient of a part of a row from the parts' sums; without one, a workgroup per row writes the
- * row's outputs. */
+ * row's outputs. Parts of GRAD_VECS groups are read in one go: what short-lived workgroups that load first
+ * move is the most this pattern of reads and writes reaches (a copy made so: 6.15 TB/s). */
+constexpr int GRAD_U = 4;
 template <int TYPE, int OP, int FEAT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, int chunk_vecs) {
     __shared__ Shared sh;
@@ -1144,45 +1146,63 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
     const bool      lead = threadIdx.x < 64;
     ListSums        ls   = {};
     Token<TYPE>     t    = {};
-    if (lead) {
-        const LossPart *p     = a.part + (long) row * a.chunks;
-        const bool      first = chunk == 0 && threadIdx.x == 0;
-        Coef            c;
-        int             id = -1;
-        if constexpr (OP != OP_DISTILL) {
-            id = a.tokens[row];
-            if (r.g && id >= 0 && id < a.n && r.mine(id))
-                t = load_token<TYPE>(a, r, row);
-            else
-                t.id = -1;
-        }
-        Sums         j  = join_parts<FEAT>(p, a.chunks, a.k);
-        const double at = p[0].a;
-        if (!j.careful)
-            rebase(j);
-        if constexpr (OP == OP_DISTILL) {
-            ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), nullptr, &j.top);
-            c  = distill_coef(a, row, ls, at, j, first);
-        } else if constexpr (OP == OP_PREFERENCE) {
-            const double d = (double) a.coef[row] * a.inv_t;
-            c              = {(float) (-d / j.s), 0.0f, 0.0f, (float) -d, d == 0.0};
-        } else {
-            c = policy_coef(a, row, id >= 0 && id < a.n, at, j, FEAT & F_ENTROPY, first);
-        }
-        if (threadIdx.x == 0) {
-            sh.sums = j;
-            sh.coef = c;
+    if constexpr (OP != OP_DISTILL)
+        t = load_token<TYPE>(a, r, row);
+    /* the first groups are on their way while the scalars are formed */
+    u32x4      raw[GRAD_U];
+    const bool some = r.g && r.v1 > r.v0;
+    if (some) {
+#pragma unroll
+        for (int i = 0; i < GRAD_U; ++i)
+            raw[i] = r.load(min(r.v0 + i * THREADS + (int) threadIdx.x, r.v1 - 1));
+    }
+    Sums j = {};
+    Coef c = {};
+    if constexpr (OP == OP_PREFERENCE) {
+        const LossRowGrad d = a.row_grad[row];
+        c                   = {d.a, 0.0f, 0.0f, d.q, d.kind == 0};
+        j.c = j.m = d.ref;
+        j.careful = d.kind == 2;
+    } else {
+        if (lead) {
+            const LossPart *p     = a.part + (long) row * a.chunks;
+            const bool      first = chunk == 0 && threadIdx.x == 0;
+            j                     = join_parts<FEAT>(p, a.chunks, a.k);
+            const double at       = p[0].a;
+            if (!j.careful)
+                rebase(j);
+            if constexpr (OP == OP_DISTILL) {
+                ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), nullptr, &j.top);
+                c  = distill_coef(a, row, ls, at, j, first);
+            } else {
+                c = policy_coef(a, row, t.id >= 0, at, j, FEAT & F_ENTROPY, first);
+            }
+            if (threadIdx.x == 0) {
+                sh.sums = j;
+                sh.coef = c;
+            }
         }
     }
     if (!r.g)
         return;
-    __syncthreads(); /* the part's special values have been read before any is written */
-    const Sums j = sh.sums;
-    const Coef c = sh.coef;
+    __syncthreads(); /* the part's values have been asked for before any is written */
+    if constexpr (OP != OP_PREFERENCE) {
+        j = sh.sums;
+        c = sh.coef;
+    }
     if (c.zero || j.careful) {
         write_rare<TYPE, FEAT, THREADS>(a, r, c, j);
     } else {
-        write_groups<TYPE, FEAT, THREADS, 4>(a, r, c, j, 0);
+        if (some) {
+#pragma unroll
+            for (int i = 0; i < GRAD_U; ++i) {
+                const int v = r.v0 + i * THREADS + (int) threadIdx.x;
+                if (v < r.v1)
+                    r.store(v, group_grad<TYPE, FEAT>(a, raw[i], keep_bits<TYPE, FEAT>(a, r, nullptr, v), c, j.c),
+                            a.streamed);
+            }
+        }
+        write_groups<TYPE, FEAT, THREADS, GRAD_U>(a, r, c, j, GRAD_U * THREADS);
         write_loose<TYPE, FEAT>(a, r, c, j);
     }
     if (c.zero)
@@ -1191,7 +1211,7 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
     if (lead) {
         if constexpr (OP == OP_DISTILL)
             write_listed<TYPE, FEAT>(a, r, List(a, lds), ls.n, c);
-        else if (threadIdx.x == 0 && t.id >= 0)
+        else if (threadIdx.x == 0 && t.id >= 0 && r.mine(t.id))
             write_token<TYPE, FEAT>(a, r, t, c, j);
     }
 }
