@@ -244,9 +244,12 @@ template <int FEAT> __device__ __forceinline__ float capped(const LossArgs &a, f
 }
 /* softcap(x) k in binary64, for the few values a row's scalars are made of */
 template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const LossArgs &a, float x) {
-    if (FEAT & F_CAP)
-        return (TYPE == GEIST_HIP_TYPE_F32 ? (double) a.cap * (double) a.k : (double) a.cap_k) *
-               tanh((double) x / (double) a.cap);
+    if (FEAT & F_CAP) {
+        if (TYPE == GEIST_HIP_TYPE_F32)
+            return (double) a.cap * (double) a.k * tanh((double) x / (double) a.cap);
+        /* (by the rounded constants the 16-bit rows' sums are made with: their rounding cancels) */
+        return (double) a.cap_k * tanh((double) x * (double) a.tanh_k * (0.5 * 0.693147180559945309417232));
+    }
     return (double) x * (double) a.k;
 }
 
@@ -339,7 +342,7 @@ template <int TYPE, int FEAT, int THREADS, int HELD> struct HeldBits {
 
 /* ---- the pass that sums --------------------------------------------------------------------- */
 /* A thread sums 2^(w - c) against a reference c of its own, the largest w of its first group: later
- * values that are larger only make larger terms, and a batch whose sum reaches 2^60 is done again
+ * values that are larger only make larger terms, and a batch whose sum reaches 2^15 is done again
  * behind a reference moved to its largest value. So the usual element costs a fused multiply-add, an
  * exponential and an addition, and no maximum. A batch of U groups is added up in binary32 by halves,
  * the batches in binary64: a running binary32 sum loses what is small beside a leading token, always
@@ -347,7 +350,7 @@ template <int TYPE, int FEAT, int THREADS, int HELD> struct HeldBits {
  * References stay above -2^20 and should stay below 2^26, where c's rounding is harmless; rows for
  * which that does not hold (nothing above -2^20, logits of 4e7 and more) are done again by
  * careful_sums. */
-constexpr float C_LOW = -1048576.0f, C_HIGH = 67108864.0f, BATCH_HIGH = 0x1p60f;
+constexpr float C_LOW = -1048576.0f, C_HIGH = 67108864.0f, BATCH_HIGH = 0x1p15f;
 struct Acc {
     float  c = C_LOW;
     double s = 0.0, t = 0.0;
