@@ -38,28 +38,39 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
         const bool      used = id >= 0 && id < a.n;
         double          lp   = 0.0;
         if (used) {
-            /* the parts joined, as join_parts does it */
-            double top = p[0].c;
-            bool   careful = p[0].careful;
-            for (int i = 1; i < a.chunks; ++i) {
-                top = fmax(top, p[i].c);
-                careful |= p[i].careful != 0;
+            /* the parts joined, as join_parts does it; four are asked for at a time */
+            double top = -1e300, s = 0.0, w = 0.0;
+            bool   careful = false, plain = false;
+            float  m = -FLT_MAX;
+            for (int i = 0; i < a.chunks; i += 4) {
+                LossPart four[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    four[k] = p[min(i + k, a.chunks - 1)];
+                if (i == 0)
+                    w = four[0].a;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i + k < a.chunks) {
+                        const LossPart &q   = four[k];
+                        const double    was = top;
+                        top                 = fmax(top, q.c);
+                        s = s * (double) __builtin_amdgcn_exp2f((float) fmax(was - top, -1e30)) +
+                            q.s * (double) __builtin_amdgcn_exp2f((float) fmax(q.c - top, -1e30));
+                        if (q.c == top) {
+                            plain = (was == top && plain) || !q.careful;
+                            m     = was == top ? m : -FLT_MAX;
+                            if (q.careful)
+                                m = fmaxf(m, q.m);
+                        }
+                        careful |= q.careful != 0;
+                    }
             }
-            float m = -FLT_MAX;
-            bool  plain = false;
-            for (int i = 0; i < a.chunks; ++i)
-                if (p[i].c == top) {
-                    plain |= p[i].careful == 0;
-                    if (p[i].careful)
-                        m = fmaxf(m, p[i].m);
-                }
             float        at  = careful ? (plain ? (float) (top / (double) a.k) : m) : (float) top;
             const double ref = careful ? (double) at * (double) a.k : (double) at;
-            double       s   = 0.0;
-            for (int i = 0; i < a.chunks; ++i)
-                s += p[i].s * (double) __builtin_amdgcn_exp2f((float) fmax(p[i].c - ref, -1e30));
+            s *= exp2(fmax(top - ref, -1e30));
             const double l2s = log2(s);
-            lp               = s == 0.0 ? -INFINITY : (p[0].a - ref - l2s) * LN2;
+            lp               = s == 0.0 ? -INFINITY : (w - ref - l2s) * LN2;
             if (lp != -INFINITY) {
                 const int side = row < edge[1] ? 0 : 1;
                 v[side] += a.ref_lp ? lp - (double) a.ref_lp[row] : lp;
