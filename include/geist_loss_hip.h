@@ -38,8 +38,9 @@ extern "C" {
  * type of the logits, rounded once; a training step that weighs the losses (a mean, an upstream
  * gradient) puts the weights into the call. NULL: loss only. It may be d_logits itself (with
  * grad_ld == ld): the rows are then replaced by their gradient. Otherwise the two must not overlap.
- * Sums over a row are formed in binary32 per thread and in binary64 across threads, everything per
- * row or per pair in binary64.
+ * Sums over a row are formed in binary32 over a few groups of 16 bytes and in binary64 beyond them,
+ * everything per row or per pair in binary64. How a row is added up follows from the call's sizes,
+ * types and options: the same call gives the same bits.
  *
  * A row that has no token left (all forbidden, or every allowed v_i is -inf) has no distribution: its loss
  * and gradient are 0. NaN or +inf among a row's allowed logits make that row's results NaN, and no
