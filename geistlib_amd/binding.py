@@ -730,6 +730,7 @@ class HipSampler:
         t.d_count = HipSampler._vector(count, rows, "torch.int32")
         t.d_weight = HipSampler._vector(weight, rows, "torch.float32")
         t.tail = int(tail)
+        t.n_rows = rows
         return t
 
     @staticmethod
@@ -746,6 +747,7 @@ class HipSampler:
         p.d_weight = HipSampler._vector(weight, n, "torch.float32")
         p.clip_low, p.clip_high = clip_low, clip_high
         p.kl_coef, p.entropy_coef = kl_coef, entropy_coef
+        p.n_rows = n
         return p
 
     @staticmethod
@@ -764,6 +766,7 @@ class HipSampler:
         p.kind = {"sigmoid": 0, "hinge": 1, "squared": 2}[kind]
         p.beta, p.margin, p.label_smoothing = beta, margin, label_smoothing
         p.length_normalised = int(length_normalised)
+        p.n_rows = tokens.shape[0]
         return p
 
     @staticmethod
@@ -772,18 +775,21 @@ class HipSampler:
 
     def distill(self, rows, teacher, loss, workspace):
         """loss: float32 [rows] or None; workspace: a device tensor of loss_workspace_bytes."""
+        assert teacher.n_rows == rows.rows, (teacher.n_rows, rows.rows)
         self._check(self.lib.geist_hip_distill_rows(self.h, C.byref(rows), C.byref(teacher),
                                                     _ptr(loss), _ptr(workspace),
                                                     self._bytes(workspace)))
 
     def policy_loss(self, rows, policy, loss, logprob, entropy, workspace):
         """loss, logprob, entropy: float32 [rows] each, or None."""
+        assert policy.n_rows == rows.rows, (policy.n_rows, rows.rows)
         self._check(self.lib.geist_hip_policy_loss_rows(
             self.h, C.byref(rows), C.byref(policy), _ptr(loss), _ptr(logprob), _ptr(entropy),
             _ptr(workspace), self._bytes(workspace)))
 
     def preference_loss(self, rows, preference, loss, ratios, logprob, workspace):
         """loss: float32 [pairs], ratios: float32 [2 pairs], logprob: float32 [rows], or None."""
+        assert preference.n_rows == rows.rows, (preference.n_rows, rows.rows)
         self._check(self.lib.geist_hip_preference_loss(
             self.h, C.byref(rows), C.byref(preference), _ptr(loss), _ptr(ratios), _ptr(logprob),
             _ptr(workspace), self._bytes(workspace)))

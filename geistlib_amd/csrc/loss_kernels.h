@@ -14,7 +14,10 @@ namespace gs {
 /* FEAT bits: what a kernel is compiled for beyond plain rows */
 constexpr int F_ENTROPY = 1; /* sum 2^u u, and a term of p_i u_i in the gradient */
 constexpr int F_CAP     = 2; /* a soft-cap */
+constexpr int F_WIDE    = 8; /* 16-bit rows: a soft-cap above CAP_SMALL, whose tanh is formed more closely */
 constexpr int F_BITS    = 4; /* an allowed-token mask or a teacher's tail: tokens that do not count */
+
+constexpr float CAP_SMALL = 64.0f;
 
 constexpr int OP_TOKEN      = 0; /* one token per row, policy loss */
 constexpr int OP_DISTILL    = 1;

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
         if (used) {
             /* the parts joined, as join_parts does it; four are asked for at a time */
             double top = -1e300, s = 0.0, w = 0.0;
-            bool   careful = false, plain = false;
+            bool   plain = false;
             float  m = -FLT_MAX;
             for (int i = 0; i < a.chunks; i += 4) {
                 LossPart four[4];
@@ -63,10 +63,10 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
                             if (q.careful)
                                 m = fmaxf(m, q.m);
                         }
-                        careful |= q.careful != 0;
                     }
             }
-            float        at  = careful ? (plain ? (float) (top / (double) a.k) : m) : (float) top;
+            const bool   careful = !plain;
+            float        at      = careful ? m : (float) top;
             const double ref = careful ? (double) at * (double) a.k : (double) at;
             s *= exp2(fmax(top - ref, -1e30));
             const double l2s = log2(s);
@@ -193,8 +193,10 @@ LossArgs args_of(const geist_hip_loss_rows &r, void *ws, bool preference = false
 }
 void launch_stage(int type, LossStage stage, int op, bool entropy, const LossArgs &a, size_t lds,
                   hipStream_t stream) {
-    const int rows = (a.cap > 0.0f ? F_CAP : 0) | (a.allowed || a.tail ? F_BITS : 0);
-    entropy        = entropy || (op == OP_TOKEN && rows == (F_CAP | F_BITS));
+    int rows = (a.cap > 0.0f ? F_CAP : 0) | (a.allowed || a.tail ? F_BITS : 0);
+    if (a.cap > CAP_SMALL && type != GEIST_HIP_TYPE_F32) /* (not a soft-cap any model has: one kernel for all) */
+        rows = F_CAP | F_WIDE | F_BITS;
+    entropy        = entropy || (op == OP_TOKEN && (rows & F_CAP) && (rows & F_BITS));
     const int feat = rows | (entropy ? F_ENTROPY : 0);
     /* without a gradient the second launch only writes the rows' outputs */
     int c = 1, v = INT32_MAX / 64;

@@ -222,11 +222,17 @@ template <int TYPE> struct Row {
 
 /* ---- values --------------------------------------------------------------------------------- */
 /* tanh(x / c) = 1 - 2 / (1 + E), E = 2^(2 x log2(e) / c): off by 1e-7 absolute, c 1e-7 in a capped
- * logit, which a 16-bit gradient does not show. For f32 rows small arguments take the odd Taylor
- * polynomial to z^13, relative error 2^-24 below 0.55. */
-__device__ __forceinline__ float cap_recip(const LossArgs &a, float x) { /* 1 / (1 + E) */
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.tanh_k));
+ * logit, which a 16-bit gradient does not show where c is what soft-caps are (up to 64). For f32 rows and
+ * larger caps small arguments take the odd Taylor polynomial to z^13, relative error 2^-24 below 0.55. */
+template <int TYPE, int FEAT> constexpr bool exact_cap = TYPE == GEIST_HIP_TYPE_F32 || (FEAT & F_WIDE) != 0;
+__device__ __forceinline__ float cap_power(const LossArgs &a, float x) { /* E */
+    return __builtin_amdgcn_exp2f(x * a.tanh_k);
 }
+__device__ __forceinline__ float cap_recip(const LossArgs &a, float x) { /* 1 / (1 + E) */
+    return __builtin_amdgcn_rcpf(1.0f + cap_power(a, x));
+}
+/* E / (1 + E)^2; an E beyond binary32 gives 0 (its r is 0) */
+__device__ __forceinline__ float cap_quarter(float E, float r) { return r * fminf(E * r, 1.0f); }
 __device__ __forceinline__ float accurate_tanh(const LossArgs &a, float x, float r) {
     const float z = x * a.inv_cap, z2 = z * z;
     float       p = 21844.0f / 6081075.0f;
@@ -245,7 +251,7 @@ template <int FEAT> __device__ __forceinline__ float capped(const LossArgs &a, f
 /* softcap(x) k in binary64, for the few values a row's scalars are made of */
 template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const LossArgs &a, float x) {
     if (FEAT & F_CAP) {
-        if (TYPE == GEIST_HIP_TYPE_F32)
+        if (exact_cap<TYPE, FEAT>)
             return (double) a.cap * (double) a.k * tanh((double) x / (double) a.cap);
         /* (by the rounded constants the 16-bit rows' sums are made with: their rounding cancels) */
         return (double) a.cap_k * tanh((double) x * (double) a.tanh_k * (0.5 * 0.693147180559945309417232));
@@ -256,23 +262,32 @@ template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const Lo
 __device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) { /* all ones or none */
     return (uint32_t) __builtin_amdgcn_sbfe((int) bits, (unsigned) i, 1u);
 }
-/* A group's exponents u = w - c, and 2^u; `keep` (masked rows, tails): bits of the tokens that count. r: what
- * the soft-cap's slope is made of. */
+/* A group's exponents u = w - c, and 2^u; `keep` (F_BITS): bits of the tokens that count. slope: a fourth of
+ * the soft-cap's, (1 - tanh^2) / 4 = E / (1 + E)^2 (as a difference of tanh from 1 it would lose its digits
+ * where it is small). */
 template <int TYPE, int FEAT>
 __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_t keep, float c,
                                            float (&e)[Elem<TYPE>::N], float (&u)[Elem<TYPE>::N],
-                                           float (&r)[Elem<TYPE>::N]) {
+                                           float (&slope)[Elem<TYPE>::N]) {
     constexpr int N = Elem<TYPE>::N;
     float         x[N];
     Elem<TYPE>::unpack(raw, x);
     if (FEAT & F_CAP) {
-        const float at = a.cap_k - c;
+        float r[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            r[i] = cap_recip(a, x[i]);
-            if (TYPE == GEIST_HIP_TYPE_F32)
+            const float E = cap_power(a, x[i]);
+            r[i]          = __builtin_amdgcn_rcpf(1.0f + E);
+            slope[i]      = cap_quarter(E, r[i]);
+        }
+        if (exact_cap<TYPE, FEAT>) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
                 u[i] = fmaf(a.cap * accurate_tanh(a, x[i], r[i]), a.k, -c);
-            else
+        } else {
+            const float at = a.cap_k - c;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
                 u[i] = fmaf(-2.0f * a.cap_k, r[i], at);
         }
     } else {
@@ -385,8 +400,8 @@ __device__ __forceinline__ float batch_sum(const LossArgs &a, float c, const u32
     for (int j = 0; j < COUNT; ++j) {
         s[j] = 0.0f;
         if ((live >> j) & 1u) {
-            float e[N], u[N], r[N];
-            group_exps<TYPE, FEAT>(a, raw[j], keep[j], c, e, u, r);
+            float e[N], u[N], slope[N];
+            group_exps<TYPE, FEAT>(a, raw[j], keep[j], c, e, u, slope);
             if (FEAT & F_ENTROPY) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
@@ -482,7 +497,7 @@ struct Sums {
 /* The sums against c = ref + log2(s) instead, rounded: s is then near 1 and the exponents of the tokens
  * that matter are small, so that they lose nothing to rounding when the gradient forms them again. */
 __device__ __forceinline__ void rebase(Sums &j) {
-    if (j.careful)
+    if (j.careful || j.s == 0.0)
         return;
     const float  c  = (float) ((double) j.c + log2(j.s));
     const double d  = (double) j.c - (double) c;
@@ -566,18 +581,19 @@ __device__ __forceinline__ Sums join_threads(Acc acc, Shared &sh) {
     j.t    = acc.t;
     return j;
 }
-__device__ __forceinline__ bool needs_care(const Sums &j) { return !(j.c < C_HIGH) || j.s == 0.0; }
-/* the parts of a row, joined by a wavefront */
+/* (a reference of a value's own has that value's 1 in its sum: less means that only C_LOW stands above the
+ * row's values, whose terms may have lost bits) */
+__device__ __forceinline__ bool needs_care(const Sums &j) { return !(j.c < C_HIGH) || j.s < 0.5; }
+/* The parts of a row, joined by a wavefront. A part that is careful beside a plain one with a larger
+ * reference weighs next to nothing: the row is plain then. */
 template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p, int chunks, float k) {
     const int lane = threadIdx.x & 63;
-    double    top = -INFINITY;
-    float     m = -FLT_MAX;
-    bool      careful = false, plain = false;
-    for (int i = lane; i < chunks; i += 64) {
+    double    top = -1e300;
+    for (int i = lane; i < chunks; i += 64)
         top = fmax(top, p[i].c);
-        careful |= p[i].careful != 0;
-    }
-    top = wave_max(top);
+    top         = wave_max(top);
+    float m     = -FLT_MAX;
+    bool  plain = false;
     for (int i = lane; i < chunks; i += 64)
         if (p[i].c == top) {
             plain |= p[i].careful == 0;
@@ -585,12 +601,9 @@ template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p
                 m = fmaxf(m, p[i].m);
         }
     Sums j    = {};
-    j.careful = __any(careful);
-    plain     = __any(plain);
-    m         = wave_max(m);
-    /* (beside a plain part with the largest reference, any m near it will do) */
-    j.m = plain ? (float) (top / (double) k) : m;
-    j.c = (float) top;
+    j.careful = !__any(plain);
+    j.m       = wave_max(m);
+    j.c       = (float) top;
     const double ref = j.ref(k);
     double s = 0.0, t = 0.0;
     for (int i = lane; i < chunks; i += 64) {
@@ -613,13 +626,14 @@ template <int TYPE, int FEAT>
 __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32_t keep, const Coef &c,
                                             float ref) {
     constexpr int N = Elem<TYPE>::N;
-    float         e[N], u[N], r[N], g[N];
-    group_exps<TYPE, FEAT>(a, raw, keep, ref, e, u, r);
+    float         e[N], u[N], slope[N], g[N];
+    group_exps<TYPE, FEAT>(a, raw, keep, ref, e, u, slope);
+    const float four = FEAT & F_CAP ? 4.0f : 1.0f, ca = four * c.a, cb = four * c.b;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        g[i] = e[i] * ((FEAT & F_ENTROPY) ? fmaf(c.b, u[i], c.a) : c.a);
-        if (FEAT & F_CAP) /* 1 - tanh^2 = 4 (r - r^2) */
-            g[i] *= 4.0f * fmaf(-r[i], r[i], r[i]);
+        g[i] = e[i] * ((FEAT & F_ENTROPY) ? fmaf(cb, u[i], ca) : ca);
+        if (FEAT & F_CAP)
+            g[i] *= slope[i];
         if ((FEAT & F_BITS) && (FEAT & F_CAP)) /* (a forbidden NaN has no slope either) */
             g[i] = __uint_as_float(__float_as_uint(g[i]) & bit_mask(keep, i));
     }
@@ -628,8 +642,8 @@ __device__ __forceinline__ u32x4 group_grad(const LossArgs &a, u32x4 raw, uint32
 template <int FEAT> __device__ __forceinline__ float cap_slope(const LossArgs &a, float x) {
     if (!(FEAT & F_CAP))
         return 1.0f;
-    const float r = cap_recip(a, x);
-    return 4.0f * fmaf(-r, r, r);
+    const float E = cap_power(a, x), r = __builtin_amdgcn_rcpf(1.0f + E);
+    return 4.0f * cap_quarter(E, r);
 }
 /* one element by any row's reference */
 template <int TYPE, int FEAT>
@@ -1037,8 +1051,7 @@ __global__ __launch_bounds__(THREADS, HELD ? 4 : 1) void k_loss_row(LossArgs a) 
     if (needs_care(j))
         j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
     if (lead) {
-        if (!j.careful)
-            rebase(j);
+        rebase(j);
         Coef c;
         if constexpr (OP == OP_DISTILL) {
             j.top    = ls.top;
@@ -1124,6 +1137,10 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
     Sums j = join_threads<FEAT, THREADS>(acc, sh);
     if (needs_care(j))
         j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
+    if (j.s == 0.0) { /* nothing counts in this part */
+        j.careful = false;
+        j.c       = C_LOW;
+    }
     if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.row_grad)
         a.row_grad[row] = {0.0f, 0.0f, 0.0f, 0}; /* (of no pair yet) */
     if (threadIdx.x == 0)
@@ -1172,8 +1189,7 @@ __global__ __launch_bounds__(THREADS) void k_loss_grad(LossArgs a, int chunks, i
             const bool      first = chunk == 0 && threadIdx.x == 0;
             j                     = join_parts<FEAT>(p, a.chunks, a.k);
             const double at       = p[0].a;
-            if (!j.careful)
-                rebase(j);
+            rebase(j);
             if constexpr (OP == OP_DISTILL) {
                 ls = read_list<TYPE, FEAT>(a, r, row, List(a, lds), nullptr, &j.top);
                 c  = distill_coef(a, row, ls, at, j, first);
@@ -1300,6 +1316,11 @@ void launch_loss(LossStage stage, int op, int feat, const LossArgs &a, size_t ld
     GS_CASE(OP_PREFERENCE, F_CAP)
     GS_CASE(OP_PREFERENCE, F_BITS)
     GS_CASE(OP_PREFERENCE, F_CAP | F_BITS)
+    if constexpr (TYPE != GEIST_HIP_TYPE_F32) {
+        GS_CASE(OP_TOKEN, F_CAP | F_WIDE | F_BITS | F_ENTROPY)
+        GS_CASE(OP_DISTILL, F_CAP | F_WIDE | F_BITS)
+        GS_CASE(OP_PREFERENCE, F_CAP | F_WIDE | F_BITS)
+    }
 #undef GS_CASE
 }
 

@@ -32,7 +32,8 @@ extern "C" {
  *   v_i = softcap(x_i) / temperature,  softcap(x) = c * tanh(x / c) for c > 0, else x,
  *   p = softmax(v) over the tokens that d_allowed allows (bit e % 32 of word
  *       d_allowed[r * allowed_ld + e / 32], allowed_ld = 0: one mask for all rows; NULL: all).
- * A forbidden token's logit is not looked at (it may be NaN) and its gradient is 0.
+ * A forbidden token's logit is not looked at (it may be NaN) and its gradient is 0 (0 or NaN in a row whose
+ * results are NaN).
  *
  * d_grad, if given, receives the gradient of the SUM of the call's losses by the logits, in the
  * type of the logits, rounded once; a training step that weighs the losses (a mean, an upstream

@@ -741,3 +741,132 @@ def test_a_batch_beyond_the_cache(hs):
     hs.sync()
     a, b = half.float(), grad[650:].float()
     assert bool(((a - b).abs() <= b.abs() * (2 * ref.HALF_STEP["bf16"] + 300 * ref.U24)).all())
+
+
+def test_masks_that_leave_a_few_tokens(hs):
+    """Most parts of a row, most wavefronts and most first groups have nothing that counts."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(31)
+    for rows, n in [(4, 130001), (70, 70000), (300, 9001)]:
+        x = logits(g, 3, n)[np.arange(rows) % 3]
+        allowed = np.zeros((rows, n), bool)
+        for r in range(rows):
+            allowed[r, g.integers(0, n, 5)] = True
+        tokens = np.array([np.flatnonzero(allowed[r])[0] for r in range(rows)], np.int32)
+        adv = g.standard_normal(rows).astype(np.float32)
+        d_tok, d_adv = dev(tokens), dev(adv)
+        start = np.array([0, rows // 2, rows], np.int32)
+        d_start = dev(start)
+        b = Batch(x, "bf16", 1, 0, allowed=allowed)
+        loss, lp, ent = out(rows), out(rows), out(rows)
+        hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, entropy_coef=0.1), loss, lp, ent, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in some_rows(rows):
+            want = ref.policy(b.x[r], "bf16", int(tokens[r]), float(adv[r]), None, None,
+                              ent=float(np.float32(0.1)), allowed=allowed[r])
+            near(ent[r].item(), want["entropy"], want["entropy_tol"] + want["entropy"] * 2.0 ** -23, f"entropy {r}")
+            near(lp[r].item(), want["logprob"], want["logprob_tol"], f"logprob {r}")
+            near(grads[r], want["grad"], want["grad_tol"], f"gradient {r}")
+        b = Batch(x, "bf16", 1, 0, allowed=allowed)
+        loss, lp = out(1), out(rows)
+        hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start, beta=0.25), loss, None, lp, b.ws)
+        hs.sync()
+        grads = b.grads()
+        if rows < 100:
+            want = ref.preference(b.x, "bf16", tokens, None, start, beta=0.25, allowed=allowed)
+            near(loss.cpu(), want["loss"], want["loss_tol"], "loss")
+            near(lp.cpu(), want["logprob"], want["logprob_tol"] + 1e-30, "logprob")
+            for r in some_rows(rows):
+                near(grads[r], want["grad"][r], want["grad_tol"][r], f"gradient {r}")
+
+
+@pytest.mark.parametrize("offset", [-1e6, -726817.6, -726900.0, -3e5, 3e5, 4.6e7, 1e9, -3.3e38, 3.3e38])
+def test_rows_far_from_zero(hs, offset):
+    """Logits at an offset of any size: what the offset leaves of their differences is what counts."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(32)
+    for rows, n in [(2, 60000), (3, 5000), (260, 2000)]:
+        x = (logits(g, rows, n) + offset).astype(np.float32)
+        tokens, adv = np.full(rows, 7, np.int32), np.ones(rows, np.float32)
+        ids, values = distill_inputs(g, rows, n, 20)
+        d_ids, d_val, d_tok, d_adv = dev(ids), dev(values), dev(tokens), dev(adv)
+        d_start = dev(np.array([0, 1, 2], np.int32))
+        b = Batch(x, "f32")
+        loss, lp, ent = out(rows), out(rows), out(rows)
+        hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, entropy_coef=0.1), loss, lp, ent, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in some_rows(rows):
+            want = ref.policy(b.x[r], "f32", 7, 1.0, None, None, ent=float(np.float32(0.1)))
+            near(lp[r].item(), want["logprob"], want["logprob_tol"] + 1e-6, f"logprob {r}")
+            near(ent[r].item(), want["entropy"], want["entropy_tol"] + 1e-6, f"entropy {r}")
+            near(grads[r], want["grad"], want["grad_tol"], f"gradient {r}")
+        for tail in (False, True):
+            hs.distill(b.view, HipSampler.teacher(d_ids, d_val, tail=tail), loss, b.ws)
+            hs.sync()
+            grads = b.grads()
+            for r in some_rows(rows):
+                want, gr, tol, g_tol = ref.distill(b.x[r], "f32", ids[r], values[r], tail)
+                near(loss[r].item(), want, tol, f"tail {tail}: loss {r}")
+                near(grads[r], gr, g_tol, f"tail {tail}: gradient {r}")
+        p_loss = out(1)
+        hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start), p_loss, None, lp, b.ws)
+        hs.sync()
+        want = ref.preference(b.x[:2], "f32", tokens[:2], None, [0, 1, 2])
+        near(p_loss.cpu(), want["loss"], want["loss_tol"], "preference loss")
+        for r in range(2):
+            near(b.grad[r].double().cpu().numpy(), want["grad"][r], want["grad_tol"][r], f"preference {r}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [2.0, 64.0, 65.0, 3e4])
+def test_soft_caps_small_and_large(hs, dtype, cap):
+    """A cap far above the logits leaves them as they are, in 16 bits too; one below them flattens them."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(33)
+    rows, n = 3, 5000
+    x = logits(g, rows, n, 4.0)
+    b = Batch(x, dtype, cap=cap)
+    tokens = np.argmax(b.x, 1).astype(np.int32)
+    d_tok, d_adv = dev(tokens), dev(np.ones(rows, np.float32))
+    loss, lp = out(rows), out(rows)
+    hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv), loss, lp, None, b.ws)
+    hs.sync()
+    grads = b.grads()
+    for r in range(rows):
+        want = ref.policy(b.x[r], dtype, int(tokens[r]), 1.0, None, None, cap=cap)
+        # (above 64 every type's small arguments are formed to 2^-24 relative: y within 64 * 2^-23)
+        slack = 64 * 2.0 ** -23 if cap > 64 else 0.0
+        tol = want["logprob_tol"] if cap <= 64 else 100 * ref.U24 + abs(want["logprob"]) * 4 * ref.U24 + slack
+        near(lp[r].item(), want["logprob"], tol, f"logprob {r}")
+        near(grads[r], want["grad"], want["grad_tol"], f"gradient {r}")
+
+
+def test_a_recorded_call_with_a_row_in_lds():
+    """A workgroup that asks for more LDS than a launch gets unasked, in a graph."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(34)
+    rows, n = 70, 200000
+    stream = torch.cuda.Stream()
+    hs = HipSampler(1, 1, stream=stream.cuda_stream)
+    base = logits(g, 2, n)[np.arange(rows) % 2]
+    b, e = Batch(base, "f32"), Batch(base, "f32")
+    ids, values = distill_inputs(g, rows, n, 30)
+    d_ids, d_val = dev(ids), dev(values)
+    t = HipSampler.teacher(d_ids, d_val, tail=True)
+    l_graph, l_eager = out(rows), out(rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        hs.distill(b.view, t, l_graph, b.ws)
+    for k in range(3):
+        b.logits.add_(0.01 * k)
+        e.logits.copy_(b.logits)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        hs.distill(e.view, t, l_eager, e.ws)
+        stream.synchronize()
+        assert torch.equal(l_graph, l_eager) and torch.equal(b.grad, e.grad), k
+    hs.close()
