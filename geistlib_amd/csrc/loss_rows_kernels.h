@@ -453,8 +453,8 @@ __device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r,
                 acc_move(c, y, a.k);
             const float u = fmaf(y, a.k, -c.c), v = __builtin_amdgcn_exp2f(u);
             c.s += (double) v;
-            if (FEAT & F_ENTROPY)
-                c.t += (double) v * (double) u;
+            if (FEAT & F_ENTROPY) /* (0 * -inf is no term, as in group_exps) */
+                c.t += (double) v * (double) fmaxf(u, -1e30f);
         }
     }
 }

@@ -1,0 +1,71 @@
+"""The losses over logit rows (include/geist_loss_hip.h) at their edges, against the binary64 statement
+(loss_reference.py) under the tolerances derived there: logits of -inf and of the type's lowest value in the
+elements outside a row's groups of 16 bytes, listed mass above 1, parts of a row without anything that counts."""
+import numpy as np
+import pytest
+
+import loss_reference as ref
+from test_gpu_loss_rows import TYPES, Batch, dev, distill_inputs, logits, near, out, some_rows
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+# rows, vocabulary, type, elements in front of the first row: one launch in groups of several sizes, and rows
+# of more than 200 000 bytes that are cut into parts; none of them a whole number of 16-byte groups
+EDGES = [(3, 5003, "f32", 1), (3, 5003, "f16", 3), (3, 5003, "bf16", 5), (300, 1001, "f32", 3), (3, 60001, "f32", 1),
+         (3, 110003, "f16", 1), (3, 110003, "bf16", 7)]
+
+
+@pytest.fixture(scope="module")
+def hs():
+    from geistlib_amd import HipSampler
+    s = HipSampler(1, 1)
+    yield s
+    s.close()
+
+
+def lowest(dtype):
+    return float(torch.finfo(TYPES[dtype]).min)
+
+
+def check_policy(hs, b, tokens, advantage, weight=None, ent=0.0, cap=0.0, temperature=1.0, allowed=None,
+                 want_entropy=True):
+    """The policy loss of every row of b (old log-probabilities: the rows' own) against the statement."""
+    from geistlib_amd import HipSampler
+    rows = b.rows
+    d = [dev(np.asarray(tokens, np.int32)), dev(np.asarray(advantage, np.float32))]
+    d_w = None if weight is None else dev(np.asarray(weight, np.float32))
+    loss, lp, H = out(rows), out(rows), out(rows) if want_entropy else None
+    hs.policy_loss(b.view, HipSampler.policy(d[0], d[1], weight=d_w, entropy_coef=ent), loss, lp, H, b.ws)
+    hs.sync()
+    grads = b.grads() if b.grad is not None else None
+    for r in some_rows(rows):
+        want = ref.policy(b.x[r], b.dtype, int(tokens[r]), float(advantage[r]), None, None,
+                          weight=1.0 if weight is None else float(np.float32(weight[r])), ent=float(np.float32(ent)),
+                          temperature=temperature, cap=cap, allowed=None if allowed is None else allowed[r])
+        near(loss[r].item(), want["loss"], want["loss_tol"], f"loss of row {r}")
+        near(lp[r].item(), want["logprob"], want["logprob_tol"] + abs(want["logprob"]) * 2.0 ** -23
+             if np.isfinite(want["logprob"]) else 0.0, f"logprob of row {r}")
+        if want_entropy:
+            near(H[r].item(), want["entropy"], want["entropy_tol"] + want["entropy"] * 2.0 ** -23, f"entropy of row {r}")
+        if grads is not None:
+            near(grads[r], want["grad"], want["grad_tol"], f"gradient of row {r}")
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows,n,dtype,lead", EDGES)
+def test_entropy_beside_logits_that_do_not_count(hs, rows, n, dtype, lead, masked):
+    """-inf and the type's lowest value at the first and the last token, which lie outside the groups: no
+    term of the entropy, and no NaN in the loss and the gradient that it is part of."""
+    g = np.random.default_rng(n + lead)
+    x = logits(g, rows, n)
+    x[0, [0, -1]] = -np.inf
+    x[1, [0, -1]] = lowest(dtype)
+    x[2, [0, 1, n // 2, -2, -1]] = -np.inf
+    allowed = None
+    if masked:
+        allowed = g.random((rows, n)) < 0.7
+        allowed[:, [0, 1, 40, -2, -1]] = True
+    for grad in ("apart", "in place", None):
+        b = Batch(x, dtype, lead, 0, grad=grad, allowed=allowed)
+        check_policy(hs, b, np.full(rows, 40), g.standard_normal(rows), ent=0.1, allowed=allowed)
