@@ -774,8 +774,9 @@ __device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has
 template <int TYPE, int FEAT>
 __device__ __forceinline__ void write_token(const LossArgs &a, const Row<TYPE> &r, const Token<TYPE> &t,
                                             const Coef &c, const Sums &j) {
-    const float u = (float) (t.template w<FEAT>(a) - j.ref(a.k));
-    const float g = __builtin_amdgcn_exp2f(u) * ((FEAT & F_ENTROPY) ? fmaf(c.b, u, c.a) : c.a) - c.q;
+    const float u = (float) (t.template w<FEAT>(a) - j.ref(a.k)); /* (-inf below binary32's lowest) */
+    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, -1e30f), c.a) : c.a;
+    const float g = __builtin_amdgcn_exp2f(u) * f - c.q;
     r.g[t.id] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, Elem<TYPE>::one(t.x)));
 }
 

@@ -69,3 +69,16 @@ def test_entropy_beside_logits_that_do_not_count(hs, rows, n, dtype, lead, maske
     for grad in ("apart", "in place", None):
         b = Batch(x, dtype, lead, 0, grad=grad, allowed=allowed)
         check_policy(hs, b, np.full(rows, 40), g.standard_normal(rows), ent=0.1, allowed=allowed)
+
+
+@pytest.mark.parametrize("ent", [0.0, 0.1])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(3, 5003), (3, 110003)])
+def test_a_token_of_the_lowest_value_with_entropy(hs, rows, n, dtype, ent):
+    """The sampled token's logit is so low that its exponent is -inf in binary32: its probability is 0, the
+    gradient at it is what the advantage makes of it, and not NaN."""
+    g = np.random.default_rng(n)
+    x = logits(g, rows, n)
+    tokens = np.array([0, n // 2, n - 1])
+    x[np.arange(3), tokens] = lowest(dtype)
+    check_policy(hs, Batch(x, dtype, 1, 0), tokens, [1.0, -0.5, 2.0], ent=ent)
