@@ -262,6 +262,9 @@ template <int TYPE, int FEAT> __device__ __forceinline__ double value64(const Lo
 __device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) { /* all ones or none */
     return (uint32_t) __builtin_amdgcn_sbfe((int) bits, (unsigned) i, 1u);
 }
+/* Where the entropy multiplies by u, u stops here: 2^u is 0 in binary32 long before, and the product with a
+ * coefficient of up to 10^35 (the weight is in it) is finite, so that 0 times it is 0. */
+constexpr float U_LOW = -1024.0f;
 /* A group's exponents u = w - c, and 2^u; `keep` (F_BITS): bits of the tokens that count. slope: a fourth of
  * the soft-cap's, (1 - tanh^2) / 4 = E / (1 + E)^2 (as a difference of tanh from 1 it would lose its digits
  * where it is small). */
@@ -307,7 +310,7 @@ __device__ __forceinline__ void group_exps(const LossArgs &a, u32x4 raw, uint32_
     if (FEAT & F_ENTROPY) { /* finite, whatever stands behind a mask: 0 * -inf is no term of an entropy */
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            u[i] = FEAT & F_BITS ? __builtin_amdgcn_fmed3f(u[i], -1e30f, 1e30f) : fmaxf(u[i], -1e30f);
+            u[i] = FEAT & F_BITS ? __builtin_amdgcn_fmed3f(u[i], U_LOW, -U_LOW) : fmaxf(u[i], U_LOW);
     }
 }
 /* Listed tokens of the workgroup's part of the row as bits (tail only): group v's start at bit
@@ -454,7 +457,7 @@ __device__ __forceinline__ void acc_loose(const LossArgs &a, const Row<TYPE> &r,
             const float u = fmaf(y, a.k, -c.c), v = __builtin_amdgcn_exp2f(u);
             c.s += (double) v;
             if (FEAT & F_ENTROPY) /* (0 * -inf is no term, as in group_exps) */
-                c.t += (double) v * (double) fmaxf(u, -1e30f);
+                c.t += (double) v * (double) fmaxf(u, U_LOW);
         }
     }
 }
@@ -529,7 +532,7 @@ __device__ __forceinline__ Sums careful_sums(const LossArgs &a, const Row<TYPE> 
             const float u = (capped<FEAT>(a, Elem<TYPE>::one(r.x[e])) - j.m) * a.k;
             const float p = __builtin_amdgcn_exp2f(u);
             s += (double) p;
-            t += (double) p * (double) fmaxf(u, -1e30f);
+            t += (double) p * (double) fmaxf(u, U_LOW);
         }
     j.s = block_reduce<THREADS, false>(s, slot);
     j.t = block_reduce<THREADS, false>(t, slot);
@@ -653,7 +656,7 @@ __device__ __forceinline__ float one_grad(const LossArgs &a, const Row<TYPE> &r,
         return 0.0f;
     const float y = capped<FEAT>(a, x);
     const float u = j.careful ? (y - j.m) * a.k : fmaf(y, a.k, -j.c);
-    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, -1e30f), c.a) : c.a;
+    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, U_LOW), c.a) : c.a;
     return __builtin_amdgcn_exp2f(u) * f * cap_slope<FEAT>(a, x);
 }
 /* the groups from v0 + `from` on, read again */
@@ -775,7 +778,7 @@ template <int TYPE, int FEAT>
 __device__ __forceinline__ void write_token(const LossArgs &a, const Row<TYPE> &r, const Token<TYPE> &t,
                                             const Coef &c, const Sums &j) {
     const float u = (float) (t.template w<FEAT>(a) - j.ref(a.k)); /* (-inf below binary32's lowest) */
-    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, -1e30f), c.a) : c.a;
+    const float f = (FEAT & F_ENTROPY) ? fmaf(c.b, fmaxf(u, U_LOW), c.a) : c.a;
     const float g = __builtin_amdgcn_exp2f(u) * f - c.q;
     r.g[t.id] = Elem<TYPE>::round(g * cap_slope<FEAT>(a, Elem<TYPE>::one(t.x)));
 }

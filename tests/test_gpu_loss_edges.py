@@ -82,3 +82,25 @@ def test_a_token_of_the_lowest_value_with_entropy(hs, rows, n, dtype, ent):
     tokens = np.array([0, n // 2, n - 1])
     x[np.arange(3), tokens] = lowest(dtype)
     check_policy(hs, Batch(x, dtype, 1, 0), tokens, [1.0, -0.5, 2.0], ent=ent)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows,n,dtype,lead", [e for e in EDGES if e[2] != "f16"])  # (it would overflow there)
+def test_large_weights_of_the_entropy(hs, rows, n, dtype, lead, masked):
+    """A weight (a loss scale) of 10^10: tokens that do not count get a gradient of 0, not 0 * inf."""
+    g = np.random.default_rng(n + 2)
+    x = logits(g, rows, n)
+    x[:, [0, 3, n // 2, -1]] = -np.inf
+    allowed = None
+    if masked:
+        allowed = g.random((rows, n)) < 0.7
+        allowed[:, [0, 3, 40, n // 2, -1]] = True
+        x[~allowed] = g.choice([np.nan, np.inf, -np.inf, 1.0], int((~allowed).sum()))
+    b = Batch(x, dtype, lead, 0, allowed=allowed)
+    check_policy(hs, b, np.full(rows, 40), g.standard_normal(rows), weight=np.full(rows, 1e10), ent=1.0,
+                 allowed=allowed)
+    # rows that are summed against a value outside the range of plain references
+    low = np.where(np.isfinite(x), x - 1e6, x)
+    b = Batch(low, "f32", lead, 0, allowed=allowed)
+    check_policy(hs, b, np.full(rows, 40), g.standard_normal(rows), weight=np.full(rows, 1e10), ent=1.0,
+                 allowed=allowed)
