@@ -755,6 +755,8 @@ __device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has
         const double ec = (double) a.entropy_coef;
         if (ec != 0.0)
             loss -= ec * H;
+        if (lp != lp) /* a spoilt row, also where no term above has seen it */
+            loss = d = lp;
         loss *= w;
         d *= w * a.inv_t;
         const double be = w * ec * a.inv_t;

@@ -104,3 +104,26 @@ def test_large_weights_of_the_entropy(hs, rows, n, dtype, lead, masked):
     b = Batch(low, "f32", lead, 0, allowed=allowed)
     check_policy(hs, b, np.full(rows, 40), g.standard_normal(rows), weight=np.full(rows, 1e10), ent=1.0,
                  allowed=allowed)
+
+
+@pytest.mark.parametrize("rows,n,dtype,lead", EDGES)
+def test_a_spoilt_row_of_any_policy_loss(hs, rows, n, dtype, lead):
+    """NaN and +inf make a row's loss, log-probability and gradient NaN also where the loss does not look at
+    the log-probability: without old ones, with an advantage of 0. Positions that are not trained on and
+    weights of 0 stay 0, and the other rows what they are."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n + 1)
+    x = logits(g, rows, n)
+    x[0, n // 3], x[1, n - 1] = np.nan, np.inf
+    d_tok, d_adv = dev(np.full(rows, 40, np.int32)), dev(np.concatenate([[1.0, 0.0], np.ones(rows - 2)]).astype(np.float32))
+    b, loss, lp = Batch(x, dtype, lead, 0), out(rows), out(rows)
+    hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv), loss, lp, None, b.ws)
+    hs.sync()
+    grads = b.grads()
+    assert np.isnan(loss[:2].cpu().numpy()).all() and np.isnan(lp[:2].cpu().numpy()).all()
+    assert np.isnan(grads[:2]).all() and (loss[2:].cpu() == -1.0).all() and np.isfinite(grads[2:]).all()
+    d_w, d_tok = dev(np.where(np.arange(rows) == 0, 0.0, 1.0).astype(np.float32)), d_tok.clone()
+    d_tok[1] = -1
+    hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, weight=d_w), loss, lp, None, b.ws)
+    hs.sync()
+    assert (loss[:2].cpu() == 0.0).all() and (b.grads()[:2] == 0).all() and lp[1].item() == 0.0
