@@ -928,15 +928,17 @@ __device__ __forceinline__ Coef distill_coef(const LossArgs &a, int row, const L
         /* sum q_j (log q_j - log p_j) */
         loss = l.q_log_q + LN2 * (l.q_sum * (l2s + (base - j.top)) - q_u);
         const double ws = w * a.inv_t;
+        /* what log S is multiplied by, q_sum + q_rest: 1 unless the listed mass exceeds it */
+        const double mass = a.tail && !(l.q_sum <= 1.0) ? l.q_sum : 1.0;
         c.a        = (float) (ws / all);
-        c.a_listed = (float) (ws / all * exp2(j.top - base));
+        c.a_listed = (float) (ws / all * mass * exp2(j.top - base));
         if (a.tail) {
-            /* p_i (1 - q_rest / p_rest) = 2^(w_i - ref) / s * (p_rest - q_rest) */
+            /* p_i (mass - q_rest / p_rest) = 2^(w_i - ref) / s * (p_rest mass - q_rest) */
             const double q_rest = l.q_sum <= 1.0 ? 1.0 - l.q_sum : l.q_sum > 1.0 ? 0.0 : l.q_sum;
             if (q_rest != 0.0)
                 loss += q_rest * (log(q_rest) -
                                   (j.s == 0.0 ? -INFINITY : LN2 * (log2(j.s) + (ref - base) - l2s)));
-            c.a = j.s == 0.0 ? 0.0f : (float) (ws * (rest / all - q_rest) / j.s);
+            c.a = j.s == 0.0 ? 0.0f : (float) (ws * (rest / all * mass - q_rest) / j.s);
         }
         loss *= w;
         c.q    = (float) ws;

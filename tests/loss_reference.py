@@ -76,6 +76,7 @@ def distill(x, dtype, ids, values, tail, temperature=1.0, cap=0.0, allowed=None,
         if tail:
             q = np.exp(val)
             rest = max(0.0, 1.0 - q.sum())
+            mass = max(1.0, q.sum())      # q.sum() + rest: what the row's log-sum is multiplied by
             out = np.ones(n, bool)
             out[at] = False
             out &= r.ok
@@ -87,10 +88,10 @@ def distill(x, dtype, ids, values, tail, temperature=1.0, cap=0.0, allowed=None,
             loss = (q * (val - r.lp[at])).sum() + (rest * (np.log(rest) - lp_rest) if rest > 0 else 0)
             share = np.exp(r.lp[out] - lp_rest) if np.isfinite(lp_rest) else 0.0
             g = np.zeros(n)
-            g[out] = r.p[out] - rest * share
-            g[at] = r.p[at] - q
-            mag[out] = r.p[out] + rest * share
-            mag[at] = r.p[at] + q
+            g[out] = mass * r.p[out] - rest * share
+            g[at] = mass * r.p[at] - q
+            mag[out] = mass * r.p[out] + rest * share
+            mag[at] = mass * r.p[at] + q
             tol = (q * (r.lp_tol[at] + (np.abs(val) + np.abs(r.lp[at])) * 4 * U24)).sum() \
                 + rest * 2 * (r.lse_tol + 4 * U24)
             # rest share sits against a reference of its own: the same bound, u from there

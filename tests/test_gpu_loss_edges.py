@@ -127,3 +127,41 @@ def test_a_spoilt_row_of_any_policy_loss(hs, rows, n, dtype, lead):
     hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, weight=d_w), loss, lp, None, b.ws)
     hs.sync()
     assert (loss[:2].cpu() == 0.0).all() and (b.grads()[:2] == 0).all() and lp[1].item() == 0.0
+
+
+@pytest.mark.parametrize("mass", [1.0, 1.01, 1.5, 8.0])
+@pytest.mark.parametrize("cap,temperature,masked", [(0.0, 1.0, False), (20.0, 0.7, True)])
+@pytest.mark.parametrize("rows,n,dtype,lead", EDGES)
+def test_distill_listed_mass_above_one(hs, rows, n, dtype, lead, cap, temperature, masked, mass):
+    """Nothing is left for the tail, and the listed mass multiplies the row's log-sum: the gradient is
+    mass p_i - q_i, and 'mass p_i' for what is not listed."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n + int(8 * mass))
+    x = logits(g, rows, n)
+    allowed = None
+    if masked:
+        allowed = g.random((rows, n)) < 0.7
+    k = 12
+    ids = np.stack([g.permutation(n)[:k] for _ in range(rows)]).astype(np.int32)
+    ids[:, 0] = np.argmax(x, 1)                   # the student's leading token among them
+    if masked:
+        for r in range(rows):
+            allowed[r, ids[r]] = True
+    q = g.random((rows, k)) + 0.05
+    values = np.log(mass * q / q.sum(1, keepdims=True)).astype(np.float32)
+    weight = g.uniform(0.2, 2, rows).astype(np.float32)
+    d_ids, d_val, d_w = dev(ids), dev(values), dev(weight)
+    t = HipSampler.teacher(d_ids, d_val, weight=d_w, tail=True)
+    for grad in ("apart", "in place"):
+        b = Batch(x, dtype, lead, 0, grad=grad, allowed=allowed, temperature=temperature, cap=cap)
+        loss = out(rows)
+        hs.distill(b.view, t, loss, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in some_rows(rows):
+            want, gr, tol, g_tol = ref.distill(b.x[r], dtype, ids[r], values[r], True, temperature, cap,
+                                               None if allowed is None else allowed[r], float(weight[r]))
+            near(loss[r].item(), want, tol, f"loss of row {r}")
+            near(grads[r], gr, g_tol, f"gradient of row {r}")
+            if grad == "apart" and not cap and dtype == "f32":   # the probabilities' slopes cancel
+                assert abs(grads[r].sum()) <= g_tol.sum()

@@ -75,3 +75,16 @@ def test_closed_forms():
     assert res["loss"] == -2.0 and res["entropy"] == pytest.approx(np.log(n))
     assert ref.preference(np.zeros((2, 4)), "f32", [0, 1], None, [0, 1, 2])["loss"][0] == pytest.approx(
         np.log(2))
+
+
+@pytest.mark.parametrize("mass", [0.9, 1.01, 1.5, 4.0])
+@pytest.mark.parametrize("cap,temperature,masked", [(0.0, 1.0, False), (5.0, 0.7, True)])
+def test_tail_gradient_for_any_listed_mass(cap, temperature, masked, mass):
+    """Above 1 nothing is left for the tail, and the loss holds the listed mass times the row's log-sum."""
+    g, x, allowed = row(11, 40)
+    allowed[[4, 9, 31]] = True
+    q = np.array([0.5, 0.3, 0.2]) * mass
+    kw = dict(tail=True, temperature=temperature, cap=cap, allowed=allowed if masked else None, weight=0.8)
+    loss = lambda z: ref.distill(z, "f32", [4, 9, 31], np.log(q), **kw)[0]  # noqa: E731
+    grad = ref.distill(x, "f32", [4, 9, 31], np.log(q), **kw)[1]
+    np.testing.assert_allclose(grad, differences(loss, x, range(40)), atol=1e-8)
