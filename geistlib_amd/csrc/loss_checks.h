@@ -20,7 +20,7 @@ namespace gs {
 struct LossPart {
     double s;       /* sum of 2^(w - c); with a teacher's tail without the listed tokens */
     double t;       /* sum of 2^u u, u = w - c (entropy only) */
-    double c;       /* the reference, near the largest w */
+    double c;       /* the reference, near the largest w; means nothing where s is 0 */
     double a;       /* chunk 0: sum of q_j (w_j - top) over the row's listed tokens; w of the sampled token */
     double listed;  /* chunk 0, tail only: sum of 2^(w_j - top) over the listed tokens */
     double top;     /* chunk 0: the largest listed w */

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void k_pair(LossArgs a) {
                     w = four[0].a;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (i + k < a.chunks) {
+                    if (i + k < a.chunks && four[k].s != 0.0) { /* (a part without a sum has no reference) */
                         const LossPart &q   = four[k];
                         const double    was = top;
                         top                 = fmax(top, q.c);

@@ -587,18 +587,20 @@ __device__ __forceinline__ Sums join_threads(Acc acc, Shared &sh) {
 /* (a reference of a value's own has that value's 1 in its sum: less means that only C_LOW stands above the
  * row's values, whose terms may have lost bits) */
 __device__ __forceinline__ bool needs_care(const Sums &j) { return !(j.c < C_HIGH) || j.s < 0.5; }
-/* The parts of a row, joined by a wavefront. A part that is careful beside a plain one with a larger
- * reference weighs next to nothing: the row is plain then. */
+/* The parts of a row, joined by a wavefront. A part in which nothing counts (its sum is 0) has no reference: it
+ * must not stand above parts whose values all lie below its own. A part that is careful beside a plain one with
+ * a larger reference weighs next to nothing: the row is plain then. */
 template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p, int chunks, float k) {
     const int lane = threadIdx.x & 63;
-    double    top = -1e300;
+    double    top  = -1e300;
     for (int i = lane; i < chunks; i += 64)
-        top = fmax(top, p[i].c);
+        if (p[i].s != 0.0)
+            top = fmax(top, p[i].c);
     top         = wave_max(top);
     float m     = -FLT_MAX;
     bool  plain = false;
     for (int i = lane; i < chunks; i += 64)
-        if (p[i].c == top) {
+        if (p[i].s != 0.0 && p[i].c == top) {
             plain |= p[i].careful == 0;
             if (p[i].careful)
                 m = fmaxf(m, p[i].m);
@@ -610,6 +612,8 @@ template <int FEAT> __device__ __forceinline__ Sums join_parts(const LossPart *p
     const double ref = j.ref(k);
     double s = 0.0, t = 0.0;
     for (int i = lane; i < chunks; i += 64) {
+        if (p[i].s == 0.0)
+            continue;
         const double d  = fmax(p[i].c - ref, -1e30);
         const double sc = (double) __builtin_amdgcn_exp2f((float) d);
         s += sc * p[i].s;
@@ -1145,10 +1149,6 @@ __global__ __launch_bounds__(THREADS) void k_loss_sums(LossArgs a) {
     Sums j = join_threads<FEAT, THREADS>(acc, sh);
     if (needs_care(j))
         j = careful_sums<TYPE, FEAT, THREADS>(a, r, map, sh.slot);
-    if (j.s == 0.0) { /* nothing counts in this part */
-        j.careful = false;
-        j.c       = C_LOW;
-    }
     if (OP == OP_PREFERENCE && chunk == 0 && threadIdx.x == 0 && a.row_grad)
         a.row_grad[row] = {0.0f, 0.0f, 0.0f, 0}; /* (of no pair yet) */
     if (threadIdx.x == 0)

@@ -165,3 +165,106 @@ def test_distill_listed_mass_above_one(hs, rows, n, dtype, lead, cap, temperatur
             near(grads[r], gr, g_tol, f"gradient of row {r}")
             if grad == "apart" and not cap and dtype == "f32":   # the probabilities' slopes cancel
                 assert abs(grads[r].sum()) <= g_tol.sum()
+
+
+@pytest.mark.parametrize("way", ["masked", "-inf"])
+@pytest.mark.parametrize("offset,temperature,dtype", [(-1e6, 1.0, "f32"), (-3e38, 1.0, "f32"), (-100.0, 1e-4, "f32"),
+                                                      (-100.0, 1e-4, "bf16"), (4.6e7, 1.0, "f32")])
+@pytest.mark.parametrize("rows,n", [(4, 130001), (300, 2001)])
+def test_parts_without_anything_that_counts(hs, rows, n, offset, temperature, dtype, way):
+    """Rows far from zero of which whole parts are masked or -inf: the empty parts, whose values are none,
+    do not stand above the others. (The larger batch has no parts and is the same rows.)"""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(41)
+    # (differences that are a few units at the call's temperature)
+    x = (logits(g, rows, n) * temperature + offset).astype(np.float32)
+    kept = np.zeros((rows, n), bool)
+    kept[0::4, :200] = True                       # the first part alone
+    kept[1::4, -300:] = True                      # the last one
+    kept[2::4, n // 2:n // 2 + 100] = True        # one between
+    kept[3::4, [5, n - 7]] = True                 # both ends
+    if way == "masked":
+        allowed, x[~kept] = kept, np.nan
+    else:
+        allowed, x[~kept] = None, -np.inf
+    tokens = np.array([np.flatnonzero(kept[r])[-1] for r in range(rows)], np.int32)
+    advantage = g.standard_normal(rows).astype(np.float32)
+    b = Batch(x, dtype, 1, 0, allowed=allowed, temperature=temperature)
+    check_policy(hs, b, tokens, advantage, ent=0.1, temperature=temperature, allowed=allowed)
+    bare = Batch(x, dtype, 1, 0, grad=None, allowed=allowed, temperature=temperature)
+    check_policy(hs, bare, tokens, advantage, ent=0.1, temperature=temperature, allowed=allowed)
+    ids = np.stack([np.flatnonzero(kept[r])[[0, -1]] for r in range(rows)]).astype(np.int32)
+    values = np.log(np.tile(np.array([0.5, 0.2]), (rows, 1))).astype(np.float32)
+    d_ids, d_val, loss = dev(ids), dev(values), out(rows)
+    for tail in (False, True):
+        hs.distill(b.view, HipSampler.teacher(d_ids, d_val, tail=tail), loss, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in some_rows(rows):
+            want, gr, tol, g_tol = ref.distill(b.x[r], dtype, ids[r], values[r], tail, temperature, 0.0,
+                                               None if allowed is None else allowed[r])
+            near(loss[r].item(), want, tol, f"tail {tail}: loss {r}")
+            near(grads[r], gr, g_tol, f"tail {tail}: gradient {r}")
+    # (a pair's sums over 300 rows are not what is looked at here)
+    b = Batch(x[:4], dtype, 1, 0, allowed=None if allowed is None else allowed[:4], temperature=temperature)
+    d_tok, d_start = dev(tokens[:4]), dev(np.array([0, 1, 4], np.int32))
+    loss, ratios, lp = out(1), out(2), out(4)
+    hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start), loss, ratios, lp, b.ws)
+    hs.sync()
+    want = ref.preference(b.x, dtype, tokens[:4], None, [0, 1, 4], temperature=temperature,
+                          allowed=None if allowed is None else allowed[:4])
+    grads = b.grads()
+    near(loss.cpu(), want["loss"], want["loss_tol"], "preference loss")
+    near(ratios.cpu(), want["ratios"], want["ratios_tol"], "ratios")
+    near(lp.cpu(), want["logprob"], want["logprob_tol"] + 1e-30, "logprob")
+    near(grads, want["grad"], want["grad_tol"], "preference gradient")
+
+
+@pytest.mark.parametrize("way", ["masked", "-inf"])
+def test_rows_cut_into_parts_that_are_all_empty(hs, way):
+    """Nothing is left in any part: no distribution, everything 0 and the token's log-probability -inf."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(42)
+    rows, n = 4, 130001
+    x = logits(g, rows, n)
+    x[1] = np.nan if way == "masked" else -np.inf
+    allowed = None
+    if way == "masked":
+        allowed = np.ones((rows, n), bool)
+        allowed[1] = False
+    tokens = np.array([3, 4, 5, n - 1], np.int32)
+    b = Batch(x, "f32", 1, 0, allowed=allowed)
+    check_policy(hs, b, tokens, [1.0, 2.0, -1.0, 0.5], ent=0.1, allowed=allowed)
+    d_ids, d_val, loss = dev(tokens[:, None].copy()), dev(np.full((rows, 1), -0.5, np.float32)), out(rows)
+    for tail in (False, True):
+        hs.distill(b.view, HipSampler.teacher(d_ids, d_val, tail=tail), loss, b.ws)
+        hs.sync()
+        assert loss[1].item() == 0.0 and (b.grads()[1] == 0).all()
+    d_tok, d_start, lp = dev(tokens), dev(np.array([0, 2, 4], np.int32)), out(rows)
+    hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start), loss[:1], None, lp, b.ws)
+    hs.sync()
+    want = ref.preference(b.x, "f32", tokens, None, [0, 2, 4], allowed=allowed)
+    near(lp.cpu(), want["logprob"], want["logprob_tol"] + 1e-30, "logprob")
+    near(loss[:1].cpu(), want["loss"], want["loss_tol"], "loss")
+    near(b.grads(), want["grad"], want["grad_tol"], "gradient")
+
+
+def test_a_spoilt_part_beside_empty_ones(hs):
+    """NaN or +inf in one part of a row whose other parts are empty: the row is NaN, the others are not."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(43)
+    rows, n = 4, 130001
+    x = np.full((rows, n), -np.inf)
+    x[:, 60000:60100] = logits(g, rows, 100)
+    x[1, 60050], x[2, 60050] = np.nan, np.inf
+    tokens = np.full(rows, 60007, np.int32)
+    b = Batch(x, "f32", 1, 0)
+    d_tok, d_adv, loss, lp = dev(tokens), dev(np.ones(rows, np.float32)), out(rows), out(rows)
+    hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv), loss, lp, None, b.ws)
+    hs.sync()
+    assert np.isnan(loss.cpu().numpy()).tolist() == [False, True, True, False]
+    assert np.isnan(b.grads()[1:3]).all() and np.isfinite(b.grads()[[0, 3]]).all()
+    d_start, two = dev(np.array([0, 1, 2, 3, 4], np.int32)), out(2)
+    hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start), two, None, lp, b.ws)
+    hs.sync()
+    assert np.isnan(two.cpu().numpy()).all() and np.isnan(lp.cpu().numpy()).tolist() == [False, True, True, False]
