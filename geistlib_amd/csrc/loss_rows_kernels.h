@@ -750,7 +750,7 @@ __device__ __forceinline__ Coef policy_coef(const LossArgs &a, int row, bool has
             loss = h < f ? -h : -f;
             d    = h < f ? 0.0 : -f;
         }
-        if (a.ref_lp) {
+        if (a.ref_lp && a.kl_coef != 0.0f) { /* (not 0 * inf) */
             const double far = (double) a.ref_lp[row] - lp;
             const double ex  = expm1(far);
             loss += (double) a.kl_coef * (ex - far);

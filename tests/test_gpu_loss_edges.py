@@ -268,3 +268,21 @@ def test_a_spoilt_part_beside_empty_ones(hs):
     hs.preference_loss(b.view, HipSampler.preference(d_tok, d_start), two, None, lp, b.ws)
     hs.sync()
     assert np.isnan(two.cpu().numpy()).all() and np.isnan(lp.cpu().numpy()).tolist() == [False, True, True, False]
+
+
+@pytest.mark.parametrize("rows,n", [(4, 5003), (4, 60001)])
+def test_a_kl_term_that_is_switched_off(hs, rows, n):
+    """kl_coef = 0 with reference log-probabilities of any value: what a call without them gives."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n)
+    b = Batch(logits(g, rows, n), "f32")
+    d_tok, d_adv = dev(np.full(rows, 9, np.int32)), dev(g.standard_normal(rows).astype(np.float32))
+    d_ref = dev(np.array([-np.inf, 1e4, 3e38, np.nan], np.float32))
+    res = []
+    for r in (None, d_ref):
+        loss = out(rows)
+        hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, ref=r, kl_coef=0.0), loss, None, None, b.ws)
+        hs.sync()
+        res.append((loss, b.grad.clone()))
+    assert bool(torch.isfinite(res[0][0]).all())
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
