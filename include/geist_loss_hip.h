@@ -44,9 +44,10 @@ extern "C" {
  * types and options: the same call gives the same bits.
  *
  * A row that has no token left (all forbidden, or every allowed v_i is -inf) has no distribution: its loss
- * and gradient are 0. NaN or +inf among a row's allowed logits make that row's results NaN, and no
- * other row's (for the preference loss: no other pair's); where a row's or pair's weight is 0,
- * loss and gradient are 0 whatever its logits are.
+ * and gradient are 0. NaN among a row's allowed logits, and without a soft-cap +inf, make that row's
+ * results NaN, and no other row's (for the preference loss: no other pair's); where a row's or pair's
+ * weight is 0, loss and gradient are 0 whatever its logits are. A soft-cap takes +inf to c and -inf to -c,
+ * both with a gradient of 0: overflowed logits of a capped model do not show in its results.
  * Limits: temperature within 1e-4 .. 1e4, logit_softcap 0 or within 1e-3 .. 1e6, at most 2^22 - 1
  * rows; GEIST_HIP_E_UNSUPPORTED where rows x the parts a row is cut into exceeds that. */
 struct geist_hip_loss_rows {

@@ -286,3 +286,62 @@ def test_a_kl_term_that_is_switched_off(hs, rows, n):
         res.append((loss, b.grad.clone()))
     assert bool(torch.isfinite(res[0][0]).all())
     assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0, 100.0])
+@pytest.mark.parametrize("rows,n,dtype,lead", EDGES)
+def test_infinite_logits(hs, rows, n, dtype, lead, cap):
+    """+inf makes its row NaN without a soft-cap; under one it is the cap itself, with no slope, as -inf is
+    the cap's negative. At the row's ends and within it.
+    With a cap of 100 other tokens' p_i reach 2^-126, below which 2^u is 0 (the instruction gives no subnormal
+    results): p_i is off by up to 2^-126 more, the gradient by that times |A| + ent (|log p_i| + H) <=
+    1 + 0.1 (2 * 100 + log n + log n) < 24 for n < 2^17, times a slope of at most 1."""
+    flushed = 24 * 2.0 ** -126
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n + 5)
+    x = logits(g, rows, n)
+    x[0, 0] = x[1, n // 2] = x[2, -1] = np.inf
+    if cap:
+        x[0, 1] = x[1, 3] = x[2, -2] = -np.inf
+    tokens = np.full(rows, 40, np.int32)
+    tokens[:3] = 0, n // 2, 7
+    ids = np.tile(np.array([0, n // 2, 7], np.int32), (rows, 1))
+    values = np.log(np.tile(np.array([0.4, 0.3, 0.1]), (rows, 1))).astype(np.float32)
+    spoilt = [] if cap else [0, 1, 2]
+    d_tok, d_adv, d_ids, d_val = dev(tokens), dev(np.ones(rows, np.float32)), dev(ids), dev(values)
+    b = Batch(x, dtype, lead, 0, cap=cap)
+    loss, lp, H = out(rows), out(rows), out(rows)
+    hs.policy_loss(b.view, HipSampler.policy(d_tok, d_adv, entropy_coef=0.1), loss, lp, H, b.ws)
+    hs.sync()
+    grads = b.grads()
+    for r in some_rows(rows):
+        if r in spoilt:
+            assert all(np.isnan(v[r].item()) for v in (loss, lp, H)) and np.isnan(grads[r]).all()
+            continue
+        want = ref.policy(b.x[r], dtype, int(tokens[r]), 1.0, None, None, ent=float(np.float32(0.1)), cap=cap)
+        near(loss[r].item(), want["loss"], want["loss_tol"], f"loss {r}")
+        near(lp[r].item(), want["logprob"], want["logprob_tol"] + abs(want["logprob"]) * 2.0 ** -23, f"logprob {r}")
+        near(H[r].item(), want["entropy"], want["entropy_tol"] + want["entropy"] * 2.0 ** -23, f"entropy {r}")
+        near(grads[r], want["grad"], want["grad_tol"] + flushed, f"gradient {r}")
+    for tail in (False, True):
+        hs.distill(b.view, HipSampler.teacher(d_ids, d_val, tail=tail), loss, b.ws)
+        hs.sync()
+        grads = b.grads()
+        for r in some_rows(rows):
+            if r in spoilt:
+                assert np.isnan(loss[r].item()) and np.isnan(grads[r]).all()
+                continue
+            want, gr, tol, g_tol = ref.distill(b.x[r], dtype, ids[r], values[r], tail, 1.0, cap)
+            near(loss[r].item(), want, tol, f"tail {tail}: loss {r}")
+            near(grads[r], gr, g_tol + flushed, f"tail {tail}: gradient {r}")
+    b = Batch(x[:3], dtype, lead, 0, cap=cap)
+    d_start, one, lp = dev(np.array([0, 1, 3], np.int32)), out(1), out(3)
+    hs.preference_loss(b.view, HipSampler.preference(d_tok[:3], d_start), one, None, lp, b.ws)
+    hs.sync()
+    if spoilt:
+        assert np.isnan(one.item()) and np.isnan(lp.cpu().numpy()).all() and np.isnan(b.grads()).all()
+    else:
+        want = ref.preference(b.x, dtype, tokens[:3], None, [0, 1, 3], cap=cap)
+        near(one.item(), want["loss"], want["loss_tol"], "preference loss")
+        near(lp.cpu(), want["logprob"], want["logprob_tol"] + np.abs(want["logprob"]) * 2.0 ** -23, "logprob")
+        near(b.grads(), want["grad"], want["grad_tol"] + flushed, "preference gradient")
