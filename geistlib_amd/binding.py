@@ -205,6 +205,21 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
 
+def _expect(ok, text):
+    """As the library refuses arguments; what only the tensors themselves can tell."""
+    if not ok:
+        raise GeistHipError(2, text)
+
+
+def _address(t, what):
+    """Address of memory that the device reaches, or None."""
+    if t is None:
+        return None
+    if not (isinstance(t, HostBuffer) or t.is_cuda or t.is_pinned()):
+        raise GeistHipError(2, what + ": not in device memory")
+    return t.data_ptr()
+
+
 class HostBuffer:
     """Page-locked host memory that the device addresses in place (geist_hip_host_malloc): pass it
     where a device tensor is expected (it has data_ptr()), read or write it through view()."""
@@ -686,49 +701,62 @@ class HipSampler:
         """The rows of a loss: logits, and grad (or None: loss only) of the same shape and type, 2-D
         float32, float16 or bfloat16 device tensors with consecutive row elements; grad may be
         logits itself. allowed: as in rows()."""
-        assert logits.dim() == 2 and logits.stride(1) == 1 or logits.shape[1] == 1
+        types = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+        def check(t, what):
+            _expect(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1),
+                    f"{what}: 2-D rows of consecutive elements, not {tuple(t.shape)} by {t.stride()}")
+            _expect(str(t.dtype) in types, f"{what}: {t.dtype}")
+        check(logits, "logits")
         r = LossRows()
-        r.type = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}[str(logits.dtype)]
-        r.d_logits = logits.data_ptr()
+        r.type = types[str(logits.dtype)]
         r.rows, r.n_vocab = logits.shape
         r.ld = logits.stride(0) if r.rows > 1 else max(logits.stride(0), r.n_vocab)
         r.temperature, r.logit_softcap = temperature, softcap
-        if allowed is not None:
-            assert allowed.dim() == 2 and allowed.stride(1) == 1 and allowed.element_size() == 4
-            assert allowed.shape[0] in (1, r.rows) and allowed.shape[1] * 32 >= r.n_vocab
-            r.d_allowed = allowed.data_ptr()
-            r.allowed_ld = 0 if allowed.shape[0] == 1 else allowed.stride(0)
         if grad is not None:
-            assert grad.shape == logits.shape and grad.dtype == logits.dtype
-            assert grad.stride(1) == 1 or grad.shape[1] == 1
-            r.d_grad = grad.data_ptr()
+            check(grad, "gradient")
+            _expect(grad.shape == logits.shape and grad.dtype == logits.dtype,
+                    f"gradient of {tuple(grad.shape)} {grad.dtype} for logits of "
+                    f"{tuple(logits.shape)} {logits.dtype}")
             r.grad_ld = grad.stride(0) if r.rows > 1 else max(grad.stride(0), r.n_vocab)
+        if allowed is not None:
+            _expect(allowed.dim() == 2 and allowed.stride(1) == 1 and allowed.element_size() == 4
+                    and allowed.shape[0] in (1, r.rows) and allowed.shape[1] * 32 >= r.n_vocab,
+                    f"allowed: {tuple(allowed.shape)} mask words of {allowed.dtype} for "
+                    f"{tuple(logits.shape)} logits")
+            r.allowed_ld = 0 if allowed.shape[0] == 1 else allowed.stride(0)
+        r.d_logits = _address(logits, "logits")
+        r.d_grad = _address(grad, "gradient")
+        r.d_allowed = _address(allowed, "allowed")
         return r
 
     @staticmethod
-    def _vector(t, n, dtype):
+    def _vector(t, n, dtype, what):
         """Device address of a vector of n values, or None."""
         if t is None:
             return None
-        assert t.shape == (n,) and (t.stride(0) == 1 or n == 1) and str(t.dtype) == dtype, \
-            (tuple(t.shape), n, t.dtype)
-        return t.data_ptr()
+        _expect(t.shape == (n,) and (t.stride(0) == 1 or n == 1) and str(t.dtype) == dtype,
+                f"{what}: {tuple(t.shape)} {t.dtype}, {n} consecutive {dtype} are needed")
+        return _address(t, what)
 
     @staticmethod
     def teacher(ids, values, count=None, weight=None, tail=False):
         """A teacher's lists: ids int32 and values float32, [rows, k]; count int32 [rows] entries of
         them that count; weight float32 [rows]. tail: values are log-probabilities, and the mass that
         is not listed counts as one more event."""
-        assert ids.shape == values.shape and ids.dim() == 2
-        assert str(ids.dtype) == "torch.int32" and str(values.dtype) == "torch.float32"
+        _expect(ids.shape == values.shape and ids.dim() == 2,
+                f"ids of {tuple(ids.shape)}, values of {tuple(values.shape)}")
+        _expect(str(ids.dtype) == "torch.int32" and str(values.dtype) == "torch.float32",
+                f"ids of {ids.dtype}, values of {values.dtype}")
         rows, k = ids.shape
-        assert (ids.stride(1) == 1 and values.stride(1) == 1) or k == 1
-        assert rows == 1 or ids.stride(0) == values.stride(0)
+        _expect((ids.stride(1) == 1 and values.stride(1) == 1) or k == 1,
+                "ids and values: lists of consecutive entries")
+        _expect(rows == 1 or ids.stride(0) == values.stride(0), "ids and values: one stride")
         t = Teacher()
-        t.d_ids, t.d_values, t.k = ids.data_ptr(), values.data_ptr(), k
+        t.d_ids, t.d_values, t.k = _address(ids, "ids"), _address(values, "values"), k
         t.ld = max(ids.stride(0), k) if rows == 1 else ids.stride(0)
-        t.d_count = HipSampler._vector(count, rows, "torch.int32")
-        t.d_weight = HipSampler._vector(weight, rows, "torch.float32")
+        t.d_count = HipSampler._vector(count, rows, "torch.int32", "count")
+        t.d_weight = HipSampler._vector(weight, rows, "torch.float32", "weight")
         t.tail = int(tail)
         t.n_rows = rows
         return t
@@ -740,11 +768,11 @@ class HipSampler:
         log-probabilities of the sampling and the reference policy (old None: the rows' own)."""
         n = tokens.shape[0]
         p = Policy()
-        p.d_tokens = HipSampler._vector(tokens, n, "torch.int32")
-        p.d_advantage = HipSampler._vector(advantage, n, "torch.float32")
-        p.d_old = HipSampler._vector(old, n, "torch.float32")
-        p.d_ref = HipSampler._vector(ref, n, "torch.float32")
-        p.d_weight = HipSampler._vector(weight, n, "torch.float32")
+        p.d_tokens = HipSampler._vector(tokens, n, "torch.int32", "tokens")
+        p.d_advantage = HipSampler._vector(advantage, n, "torch.float32", "advantage")
+        p.d_old = HipSampler._vector(old, n, "torch.float32", "old")
+        p.d_ref = HipSampler._vector(ref, n, "torch.float32", "ref")
+        p.d_weight = HipSampler._vector(weight, n, "torch.float32", "weight")
         p.clip_low, p.clip_high = clip_low, clip_high
         p.kl_coef, p.entropy_coef = kl_coef, entropy_coef
         p.n_rows = n
@@ -756,40 +784,71 @@ class HipSampler:
         """Pairs of sequences: tokens int32 [rows] (-1: not counted), seq_start int32 [2 pairs + 1],
         ref float32 [rows] log-probabilities of the reference model, weight float32 [pairs]. kind:
         "sigmoid", "hinge" or "squared"."""
-        n_pairs = (seq_start.shape[0] - 1) // 2
+        n, n_pairs = tokens.shape[0], (seq_start.shape[0] - 1) // 2
+        _expect(n_pairs > 0, f"seq_start: {seq_start.shape[0]} entries, 2 pairs + 1 are needed")
         p = Preference()
-        p.d_tokens = HipSampler._vector(tokens, tokens.shape[0], "torch.int32")
-        p.d_ref = HipSampler._vector(ref, tokens.shape[0], "torch.float32")
-        p.d_seq_start = HipSampler._vector(seq_start, 2 * n_pairs + 1, "torch.int32")
+        p.d_tokens = HipSampler._vector(tokens, n, "torch.int32", "tokens")
+        p.d_ref = HipSampler._vector(ref, n, "torch.float32", "ref")
+        p.d_seq_start = HipSampler._vector(seq_start, 2 * n_pairs + 1, "torch.int32", "seq_start")
         p.n_pairs = n_pairs
-        p.d_weight = HipSampler._vector(weight, n_pairs, "torch.float32")
+        p.d_weight = HipSampler._vector(weight, n_pairs, "torch.float32", "weight")
         p.kind = {"sigmoid": 0, "hinge": 1, "squared": 2}[kind]
         p.beta, p.margin, p.label_smoothing = beta, margin, label_smoothing
         p.length_normalised = int(length_normalised)
-        p.n_rows = tokens.shape[0]
+        p.n_rows = n
         return p
 
     @staticmethod
-    def _bytes(t):
-        return t.numel() * t.element_size() if t is not None else 0
+    def _output(t, n, what):
+        """Address of what a loss writes n float32 to: a contiguous device tensor or a HostBuffer with
+        room for them, or None."""
+        if t is None:
+            return None
+        # (texts are formed where they are needed: a call is a few microseconds)
+        if isinstance(t, HostBuffer):
+            ok = t.nbytes >= 4 * n
+        else:
+            ok = t.numel() >= n and t.is_contiguous() and str(t.dtype) == "torch.float32"
+        if not ok:
+            has = f"{t.nbytes} bytes" if isinstance(t, HostBuffer) else f"{tuple(t.shape)} {t.dtype}"
+            raise GeistHipError(2, f"{what}: {has}, {n} consecutive torch.float32 are needed")
+        return _address(t, what)
+
+    @staticmethod
+    def _scratch(t):
+        """Address and bytes of a workspace."""
+        if t is None:
+            return None, 0
+        _expect(t.is_contiguous(), "workspace: not contiguous")
+        return _address(t, "workspace"), t.numel() * t.element_size()
+
+    @staticmethod
+    def _same_rows(what, rows):
+        if what.n_rows != rows.rows:
+            raise GeistHipError(2, f"{what.n_rows} rows of {type(what).__name__.lower()} for "
+                                   f"{rows.rows} rows of logits")
 
     def distill(self, rows, teacher, loss, workspace):
         """loss: float32 [rows] or None; workspace: a device tensor of loss_workspace_bytes."""
-        assert teacher.n_rows == rows.rows, (teacher.n_rows, rows.rows)
-        self._check(self.lib.geist_hip_distill_rows(self.h, C.byref(rows), C.byref(teacher),
-                                                    _ptr(loss), _ptr(workspace),
-                                                    self._bytes(workspace)))
+        self._same_rows(teacher, rows)
+        self._check(self.lib.geist_hip_distill_rows(
+            self.h, C.byref(rows), C.byref(teacher), self._output(loss, rows.rows, "loss"),
+            *self._scratch(workspace)))
 
     def policy_loss(self, rows, policy, loss, logprob, entropy, workspace):
         """loss, logprob, entropy: float32 [rows] each, or None."""
-        assert policy.n_rows == rows.rows, (policy.n_rows, rows.rows)
+        self._same_rows(policy, rows)
+        n = rows.rows
         self._check(self.lib.geist_hip_policy_loss_rows(
-            self.h, C.byref(rows), C.byref(policy), _ptr(loss), _ptr(logprob), _ptr(entropy),
-            _ptr(workspace), self._bytes(workspace)))
+            self.h, C.byref(rows), C.byref(policy), self._output(loss, n, "loss"),
+            self._output(logprob, n, "logprob"), self._output(entropy, n, "entropy"),
+            *self._scratch(workspace)))
 
     def preference_loss(self, rows, preference, loss, ratios, logprob, workspace):
         """loss: float32 [pairs], ratios: float32 [2 pairs], logprob: float32 [rows], or None."""
-        assert preference.n_rows == rows.rows, (preference.n_rows, rows.rows)
+        self._same_rows(preference, rows)
+        n = preference.n_pairs
         self._check(self.lib.geist_hip_preference_loss(
-            self.h, C.byref(rows), C.byref(preference), _ptr(loss), _ptr(ratios), _ptr(logprob),
-            _ptr(workspace), self._bytes(workspace)))
+            self.h, C.byref(rows), C.byref(preference), self._output(loss, n, "loss"),
+            self._output(ratios, 2 * n, "ratios"), self._output(logprob, rows.rows, "logprob"),
+            *self._scratch(workspace)))

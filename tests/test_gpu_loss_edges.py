@@ -345,3 +345,42 @@ def test_infinite_logits(hs, rows, n, dtype, lead, cap):
         near(one.item(), want["loss"], want["loss_tol"], "preference loss")
         near(lp.cpu(), want["logprob"], want["logprob_tol"] + np.abs(want["logprob"]) * 2.0 ** -23, "logprob")
         near(b.grads(), want["grad"], want["grad_tol"] + flushed, "preference gradient")
+
+
+def test_outputs_without_room_are_refused(hs):
+    """A vector that is too short or of another type is refused before anything is written; page-locked host
+    memory is taken like device memory."""
+    from geistlib_amd import HipSampler
+    from geistlib_amd.binding import GeistHipError
+    rows, n = 4, 1000
+    b = Batch(logits(np.random.default_rng(50), rows, n), "f32")
+    d_tok, d_adv = dev(np.full(rows, 9, np.int32)), dev(np.ones(rows, np.float32))
+    d_ids, d_val = dev(np.full((rows, 1), 9, np.int32)), dev(np.zeros((rows, 1), np.float32))
+    d_start = dev(np.array([0, 1, 2, 3, 4], np.int32))
+    p, q = HipSampler.policy(d_tok, d_adv), HipSampler.preference(d_tok, d_start)
+    t = HipSampler.teacher(d_ids, d_val)
+    ok, short, other = out(rows), out(rows)[:rows - 1], torch.full((rows,), -77.0, dtype=torch.float16, device="cuda")
+    other_rows, small = HipSampler.policy(d_tok[:3], d_adv[:3]), hs.host_buffer(4)
+    for bad in (short, other, torch.zeros(rows), small):
+        for call in (lambda: hs.distill(b.view, t, bad, b.ws),
+                     lambda: hs.policy_loss(b.view, p, bad, None, None, b.ws),
+                     lambda: hs.policy_loss(b.view, p, ok, bad, None, b.ws),
+                     lambda: hs.policy_loss(b.view, p, ok, None, bad, b.ws),
+                     lambda: hs.preference_loss(b.view, q, ok, bad, None, b.ws),
+                     lambda: hs.preference_loss(b.view, q, ok, None, bad, b.ws),
+                     lambda: hs.preference_loss(b.view, q, bad[:1] if torch.is_tensor(bad) else small, None, None, b.ws),
+                     lambda: hs.policy_loss(b.view, other_rows, ok, None, None, b.ws)):
+            with pytest.raises(GeistHipError) as err:
+                call()
+            assert err.value.code == 2
+    hs.sync()
+    assert (ok.cpu() == -77.0).all() and (short.cpu() == -77.0).all() and (other.cpu() == -77.0).all()
+    assert (b.grads() == 7.0).all()
+    hs.policy_loss(b.view, p, None, ok, None, b.ws)
+    host, pinned = hs.host_buffer(4 * rows), torch.zeros(rows).pin_memory()
+    hs.policy_loss(b.view, p, None, host, None, b.ws)
+    hs.policy_loss(b.view, p, None, pinned, None, b.ws)
+    hs.sync()
+    assert (host.view(np.float32) == ok.cpu().numpy()).all() and torch.equal(pinned, ok.cpu())
+    host.close()
+    small.close()
