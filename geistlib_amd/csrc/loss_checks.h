@@ -95,8 +95,9 @@ __attribute__((format(printf, 3, 4))) inline int refuse(Refusal &why, int code, 
     return code;
 }
 
+/* result: one of the vectors that the call writes beside the gradient, if any */
 inline int check_loss_rows(const geist_hip_loss_rows *r, const void *ws, size_t ws_bytes,
-                           const float *loss, Refusal &why) {
+                           const float *result, Refusal &why) {
     if (!r || !r->d_logits)
         return refuse(why, GEIST_HIP_E_INVALID_ARG, "null rows or logits");
     if (r->type != GEIST_HIP_TYPE_F32 && r->type != GEIST_HIP_TYPE_F16 && r->type != GEIST_HIP_TYPE_BF16)
@@ -141,8 +142,8 @@ inline int check_loss_rows(const geist_hip_loss_rows *r, const void *ws, size_t 
         return refuse(why, GEIST_HIP_E_INVALID_ARG,
                       "workspace: %zu bytes, 16-byte aligned, are needed (%zu given)", need,
                       ws ? ws_bytes : (size_t) 0);
-    if (!loss && !r->d_grad)
-        return refuse(why, GEIST_HIP_E_INVALID_ARG, "neither a loss nor a gradient is asked for");
+    if (!result && !r->d_grad)
+        return refuse(why, GEIST_HIP_E_INVALID_ARG, "neither a result nor a gradient is asked for");
     return GEIST_HIP_OK;
 }
 

@@ -2573,8 +2573,10 @@ int geist_hip_policy_loss_rows(geist_hip_sampler *s, const struct geist_hip_loss
                                size_t workspace_bytes) {
     if (!s)
         return GEIST_HIP_E_INVALID_ARG;
-    Refusal why;
-    int     rc = check_loss_rows(rows, d_workspace, workspace_bytes, d_loss, why);
+    Refusal      why;
+    /* (without a loss and a gradient the rows are scored) */
+    const float *result = d_loss ? d_loss : d_logprob ? d_logprob : d_entropy;
+    int          rc     = check_loss_rows(rows, d_workspace, workspace_bytes, result, why);
     if (rc == GEIST_HIP_OK)
         rc = check_policy(policy, why);
     if (rc != GEIST_HIP_OK)
@@ -2590,8 +2592,9 @@ int geist_hip_preference_loss(geist_hip_sampler *s, const struct geist_hip_loss_
                               size_t workspace_bytes) {
     if (!s)
         return GEIST_HIP_E_INVALID_ARG;
-    Refusal why;
-    int     rc = check_loss_rows(rows, d_workspace, workspace_bytes, d_loss, why);
+    Refusal      why;
+    const float *result = d_loss ? d_loss : d_ratios ? d_ratios : d_logprob;
+    int          rc     = check_loss_rows(rows, d_workspace, workspace_bytes, result, why);
     if (rc == GEIST_HIP_OK)
         rc = check_preference(preference, why);
     if (rc != GEIST_HIP_OK)

@@ -105,8 +105,9 @@ int geist_hip_distill_rows(geist_hip_sampler *s, const struct geist_hip_loss_row
  * advantage of 0 gives 0 whatever the ratio. Tokens outside [0, n_vocab) mark positions that are
  * not trained on (prompt, padding): loss, logprob and gradient 0, H is still reported. A token
  * with probability 0 (forbidden, or a logit of -inf) has logprob -inf and loss and gradient 0.
- * d_loss may be NULL when d_grad is given; d_logprob ([rows], lp) and d_entropy ([rows], H) may be
- * NULL. With d_ref = NULL, kl_coef must be 0. */
+ * d_loss, d_logprob ([rows], lp), d_entropy ([rows], H) and d_grad may each be NULL, not all of them:
+ * d_logprob alone scores the tokens. With d_ref = NULL, kl_coef must be 0; with kl_coef = 0, d_ref is
+ * not looked at. */
 struct geist_hip_policy {
     const int32_t *d_tokens;    /* [rows] */
     const float   *d_advantage; /* [rows] */
@@ -136,8 +137,8 @@ int geist_hip_policy_loss_rows(geist_hip_sampler *s, const struct geist_hip_loss
  * Rows whose token is outside [0, n_vocab) (prompt, padding) and rows that give their token
  * probability 0 are left out of the sums: logprob 0 or -inf, gradient 0. Rows in front of the first
  * sequence and behind the last are not read, and their logprob and gradient are not written.
- * d_loss [n_pairs] may be NULL when d_grad is given; d_ratios [2 * n_pairs] (D_s) and d_logprob
- * [rows] may be NULL. */
+ * d_loss [n_pairs], d_ratios [2 * n_pairs] (D_s), d_logprob [rows] and d_grad may each be NULL, not
+ * all of them. */
 #define GEIST_HIP_PREFERENCE_SIGMOID 0
 #define GEIST_HIP_PREFERENCE_HINGE 1
 #define GEIST_HIP_PREFERENCE_SQUARED 2

@@ -384,3 +384,32 @@ def test_outputs_without_room_are_refused(hs):
     assert (host.view(np.float32) == ok.cpu().numpy()).all() and torch.equal(pinned, ok.cpu())
     host.close()
     small.close()
+
+
+@pytest.mark.parametrize("rows,n,dtype,lead", [(3, 5003, "f32", 1), (3, 110003, "bf16", 7), (300, 1001, "f16", 3)])
+def test_scores_alone(hs, rows, n, dtype, lead):
+    """Log-probabilities, entropies or ratios without a loss and without a gradient: the bits of a call that
+    asks for the loss too."""
+    from geistlib_amd import HipSampler
+    g = np.random.default_rng(n + 9)
+    b = Batch(logits(g, rows, n), dtype, lead, 0, grad=None)
+    d_tok, d_adv = dev(g.integers(0, n, rows).astype(np.int32)), dev(np.ones(rows, np.float32))
+    p = HipSampler.policy(d_tok, d_adv)
+    loss, lp, H = out(rows), out(rows), out(rows)
+    hs.policy_loss(b.view, p, loss, lp, H, b.ws)
+    lp2, H2 = out(rows), out(rows)
+    hs.policy_loss(b.view, p, None, lp2, H2, b.ws)
+    hs.sync()
+    assert torch.equal(lp, lp2) and torch.equal(H, H2)
+    H3 = out(rows)
+    hs.policy_loss(b.view, p, None, None, H3, b.ws)
+    hs.sync()
+    assert torch.equal(H, H3)
+    d_start = dev(np.array([0, rows // 3, rows], np.int32))
+    q = HipSampler.preference(d_tok, d_start)
+    one, ratios, lp = out(1), out(2), out(rows)
+    hs.preference_loss(b.view, q, one, ratios, lp, b.ws)
+    ratios2, lp2 = out(2), out(rows)
+    hs.preference_loss(b.view, q, None, ratios2, lp2, b.ws)
+    hs.sync()
+    assert torch.equal(ratios, ratios2) and torch.equal(lp, lp2)
