@@ -2,6 +2,7 @@
 (`tensor.data_ptr()`); nothing here computes on logits."""
 import ctypes as C
 import os
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -804,51 +805,62 @@ class HipSampler:
         room for them, or None."""
         if t is None:
             return None
-        # (texts are formed where they are needed: a call is a few microseconds)
-        if isinstance(t, HostBuffer):
-            ok = t.nbytes >= 4 * n
-        else:
-            ok = t.numel() >= n and t.is_contiguous() and str(t.dtype) == "torch.float32"
-        if not ok:
-            has = f"{t.nbytes} bytes" if isinstance(t, HostBuffer) else f"{tuple(t.shape)} {t.dtype}"
+        # (in one expression, and texts only where they are needed: a call is a few microseconds)
+        if t.__class__ is HostBuffer:
+            if t.nbytes >= 4 * n:
+                return t.data_ptr()
+        elif (t.dtype is sys.modules["torch"].float32 and t.nbytes >= 4 * n and t.is_contiguous()
+              and (t.is_cuda or t.is_pinned())):
+            return t.data_ptr()
+        has = f"{t.nbytes} bytes" if isinstance(t, HostBuffer) else f"{tuple(t.shape)} {t.dtype}"
+        if isinstance(t, HostBuffer) or t.numel() < n or not t.is_contiguous() or str(t.dtype) != "torch.float32":
             raise GeistHipError(2, f"{what}: {has}, {n} consecutive torch.float32 are needed")
-        return _address(t, what)
+        raise GeistHipError(2, f"{what}: not in device memory")
 
     @staticmethod
     def _scratch(t):
         """Address and bytes of a workspace."""
         if t is None:
             return None, 0
-        _expect(t.is_contiguous(), "workspace: not contiguous")
-        return _address(t, "workspace"), t.numel() * t.element_size()
+        if t.is_contiguous() and (t.is_cuda or t.is_pinned()):
+            return t.data_ptr(), t.nbytes
+        raise GeistHipError(2, "workspace: " + ("not in device memory" if t.is_contiguous() else "not contiguous"))
 
     @staticmethod
-    def _same_rows(what, rows):
-        if what.n_rows != rows.rows:
-            raise GeistHipError(2, f"{what.n_rows} rows of {type(what).__name__.lower()} for "
-                                   f"{rows.rows} rows of logits")
+    def _other_rows(what, rows):
+        return GeistHipError(2, f"{what.n_rows} rows of {type(what).__name__.lower()} for {rows.rows} rows of logits")
 
+    # (the structures go as they are: by their argument types, ctypes passes their addresses)
     def distill(self, rows, teacher, loss, workspace):
         """loss: float32 [rows] or None; workspace: a device tensor of loss_workspace_bytes."""
-        self._same_rows(teacher, rows)
-        self._check(self.lib.geist_hip_distill_rows(
-            self.h, C.byref(rows), C.byref(teacher), self._output(loss, rows.rows, "loss"),
-            *self._scratch(workspace)))
+        n = rows.rows
+        if teacher.n_rows != n:
+            raise self._other_rows(teacher, rows)
+        scratch, room = self._scratch(workspace)
+        rc = self.lib.geist_hip_distill_rows(self.h, rows, teacher, self._output(loss, n, "loss"), scratch, room)
+        if rc:
+            self._check(rc)
 
     def policy_loss(self, rows, policy, loss, logprob, entropy, workspace):
         """loss, logprob, entropy: float32 [rows] each, or None."""
-        self._same_rows(policy, rows)
-        n = rows.rows
-        self._check(self.lib.geist_hip_policy_loss_rows(
-            self.h, C.byref(rows), C.byref(policy), self._output(loss, n, "loss"),
-            self._output(logprob, n, "logprob"), self._output(entropy, n, "entropy"),
-            *self._scratch(workspace)))
+        output, n = self._output, rows.rows
+        if policy.n_rows != n:
+            raise self._other_rows(policy, rows)
+        scratch, room = self._scratch(workspace)
+        rc = self.lib.geist_hip_policy_loss_rows(
+            self.h, rows, policy, output(loss, n, "loss"), output(logprob, n, "logprob"),
+            output(entropy, n, "entropy"), scratch, room)
+        if rc:
+            self._check(rc)
 
     def preference_loss(self, rows, preference, loss, ratios, logprob, workspace):
         """loss: float32 [pairs], ratios: float32 [2 pairs], logprob: float32 [rows], or None."""
-        self._same_rows(preference, rows)
-        n = preference.n_pairs
-        self._check(self.lib.geist_hip_preference_loss(
-            self.h, C.byref(rows), C.byref(preference), self._output(loss, n, "loss"),
-            self._output(ratios, 2 * n, "ratios"), self._output(logprob, rows.rows, "logprob"),
-            *self._scratch(workspace)))
+        output, n = self._output, preference.n_pairs
+        if preference.n_rows != rows.rows:
+            raise self._other_rows(preference, rows)
+        scratch, room = self._scratch(workspace)
+        rc = self.lib.geist_hip_preference_loss(
+            self.h, rows, preference, output(loss, n, "loss"), output(ratios, 2 * n, "ratios"),
+            output(logprob, rows.rows, "logprob"), scratch, room)
+        if rc:
+            self._check(rc)
