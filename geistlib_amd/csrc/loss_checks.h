@@ -49,7 +49,8 @@ enum LossUse { LOSS_ALONE, LOSS_AND_GRADIENT, LOSS_PREFERENCE };
  * logit once; two launches over parts of the rows read them twice and pay a launch more, but spread a few
  * long rows over the device. Measured, one launch against two (us):
  *   with a gradient  1 x 262 KB 15.3 / 8.4, 32 x 257 KB about equal, 16 x 524 KB 30.1 / 12.4,
- *                    64 x 513 KB 25.4 / 20.2 (with a list 26.3 / 32.4), 128 x 513 KB 35.5 / 43.1
+ *                    64 x 513 KB 25.4 / 20.2 (with a list 26.3 / 32.4, which the rule does not look at: distillation of
+ *                    33 to 64 such rows pays for it), 128 x 513 KB 35.5 / 43.1
  *   loss alone       1 x 257 KB 8.1 / 7.4, 64 x 257 KB 9.2 / 9.6, 16 x 524 KB 13.5 / 8.2, 128 x 524 KB 17.0 / 17.3
  * The preference loss has its sums and its gradient in two launches whatever the sizes; its parts of 64 KB
  * cost a large batch nothing (1760 x 257 KB: 264 us whole, 267 cut) and spread a small one
